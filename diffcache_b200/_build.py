@@ -9,14 +9,15 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(_HERE, "csrc")
 LIB_DIR = os.path.join(_HERE, "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "libdiffcache_b200.so")
-SOURCES = ["scan.cu", "scan_tc.cu", "select.cu", "attend.cu", "pq.cu", "budget.cu", "exchange.cu", "engine.cu"]
-HEADERS = [os.path.join(CSRC, "common.cuh"), os.path.join(CSRC, "exchange.cuh"),
+SOURCES = ["scan.cu", "scan_tc.cu", "select.cu", "attend.cu", "pq.cu", "budget.cu", "exchange.cu",
+           "quant.cu", "scan_q4.cu", "attend_q4.cu", "engine.cu"]
+HEADERS = [os.path.join(CSRC, "common.cuh"), os.path.join(CSRC, "exchange.cuh"), os.path.join(CSRC, "q4.cuh"),
            os.path.join(_HERE, "..", "include", "diffcache_b200.h")]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC", "-shared", "--threads=0",
 ]
 
 

@@ -16,15 +16,24 @@ SIGNATURES = {
     "dc_last_error": (ctypes.c_char_p, []),
     "dc_version": (_i32, []),
     "dc_create": (_i32, [_i32, _i32, _i32, _i32, _i64, _i32, _i32, ctypes.POINTER(_vp)]),
+    "dc_create_q4": (_i32, [_i32, _i32, _i32, _i32, _i64, _i32, _i32, ctypes.POINTER(_vp)]),
+    "dc_store_bits": (_i32, [_vp]),
     "dc_destroy": (_i32, [_vp]),
     "dc_set_row_offset": (_i32, [_vp, _i64]),
     "dc_prefill": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _u64]),
     "dc_insert": (_i32, [_vp, _vp, _vp, _u64]),
+    "dc_write_rows": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _u64]),
+    "dc_read_rows": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _u64]),
+    "dc_score_rows": (_i32, [_vp, _vp, _i32, _i64, _vp, _i64, _u64]),
+    "dc_attend_rows": (_i32, [_vp, _vp, _i64, _vp, _i32, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i32, _f32, _vp, _vp,
+                              _u64]),
     "dc_ctx_len": (_i32, [_vp, ctypes.POINTER(_i64)]),
     "dc_query": (_i32, [_vp, _vp, _i32, _vp, _vp, _vp, _vp, _u64]),
     "dc_check_status": (_i32, [_vp, _u64]),
     "dc_get_keys": (_i32, [_vp, _vp]),
     "dc_export_rows": (_i32, [_vp, _vp, _vp]),
+    "dc_export_q4": (_i32, [_vp, _vp, _vp, _vp, _vp]),
+    "dc_import_q4": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64]),
     "dc_update_r_sq": (_i32, [_vp, _vp, _i32]),
     "dc_decode_attend": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _f32, _vp, _vp, _vp, _u64]),
     "dc_decode_attend_strided": (_i32, [_vp, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i32, _i32, _f32, _vp, _vp,
@@ -72,6 +81,13 @@ SIGNATURES = {
                                         _vp, _vp, _vp, _vp, _i64, _i64, _i32, _f32, _vp, _vp, _vp, _vp, _u64]),
     "dc_lse_combine": (_i32, [_vp, _i64, _vp, _i64, _i32, _i64, _i32, _i32, _vp, _vp, _u64]),
     "dc_gather_rows": (_i32, [_vp, _i64, _i32, _i32, _vp, _i64, _i32, _vp, _u64]),
+    "dc_q4_write_rows": (_i32, [_vp, _vp, _i64, _i64, _i64, _i32, _i32, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _i64, _i64,
+                                _u64]),
+    "dc_q4_read_rows": (_i32, [_vp, _vp, _i64, _i64, _i32, _i32, _i32, _i64, _vp, _i64, _i64, _vp, _u64]),
+    "dc_q4_score_scan": (_i32, [_vp, _vp, _i64, _i32, _i64, _i32, _i32, _vp, _i32, _i32, _vp, _i64, _vp, _u64]),
+    "dc_q4_attend": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _i64, _i32, _i64, _vp,
+                            _vp, _vp, _vp, _vp, _i64, _i64, _i32, _f32, _vp, _vp, _vp, _vp, _vp, _u64]),
+    "dc_q4_attend_scratch_bytes": (_i64, [_i32, _i32, _i32]),
     "dc_pq_build_lut": (_i32, [_vp, _i32, _i32, _i32, _vp, _i32, _i32, _i32, _vp, _u64]),
     "dc_pq_adc_scan": (_i32, [_vp, _i64, _i32, _i64, _i32, _vp, _vp, _i64, _vp, _u64]),
     "dc_rerank_scores": (_i32, [_vp, _i64, _i32, _i32, _i32, _vp, _i32, _i32, _vp, _i64, _i32, _vp, _u64]),

@@ -432,13 +432,14 @@ constexpr int kCombineMaxParts = 1024;
 
 // One row (blockIdx.x) of a merge.  xepoch: epoch the fan-out stores carry (xo.world != 0); want: epoch the polled
 // parts must carry (ll.chan != nullptr).  Uses static shared memory: a kernel that calls it twice separates the
-// calls with a block barrier.
+// calls with a block barrier.  keep_nan: a sum that is NaN (a NaN in an attended row) gives NaN, as the formula
+// does; otherwise it counts as an empty row.
 template <int DT>
 __device__ __forceinline__ void
 combine_row(const float* __restrict__ part_acc, int64_t acc_ps, int64_t acc_rs, const float* __restrict__ part_ml,
             int64_t ml_ps, int64_t ml_rs, int n_part, int dim, uint16_t* __restrict__ out, float* __restrict__ out_lse,
             float* __restrict__ out_acc, float* __restrict__ out_ml, const XchgLL& ll, int64_t ll_ml_off, uint32_t want,
-            const XchgOut& xo, int64_t xo_ml_off, uint32_t xepoch) {
+            const XchgOut& xo, int64_t xo_ml_off, uint32_t xepoch, bool keep_nan) {
     const int64_t row = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     __shared__ float s_w[kCombineMaxParts];   // weight of every part: exp2(m_s - M)
@@ -520,6 +521,7 @@ combine_row(const float* __restrict__ part_acc, int64_t acc_ps, int64_t acc_rs, 
     }
     __syncthreads();
     const float L = s_L;
+    const bool some = keep_nan ? !(L <= 0.0f) : L > 0.0f;
     const bool vec_ok = (dim % 4 == 0) && (dim / 4 <= kCombineThreads) && (kCombineThreads % (dim / 4) == 0) &&
                         (acc_ps % 4 == 0) && ((reinterpret_cast<uintptr_t>(acc) & 15) == 0);
     if (vec_ok) {
@@ -547,7 +549,7 @@ combine_row(const float* __restrict__ part_acc, int64_t acc_ps, int64_t acc_rs, 
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const int d = 4 * tid + j;
-                e4[j] = float_to_elem<DT>(L > 0.0f ? v4[j] / L : 0.0f);
+                e4[j] = float_to_elem<DT>(some ? v4[j] / L : 0.0f);
                 if (out) out[row * dim + d] = e4[j];
                 if (out_acc) out_acc[row * dim + d] = v4[j];
             }
@@ -566,14 +568,14 @@ combine_row(const float* __restrict__ part_acc, int64_t acc_ps, int64_t acc_rs, 
         for (int d = tid; d < dim; d += kCombineThreads) {
             float o = 0.0f;
             for (int s = 0; s < n_part; s++) o += acc[s * acc_ps + d] * s_w[s];
-            if (out) out[row * dim + d] = float_to_elem<DT>(L > 0.0f ? o / L : 0.0f);
+            if (out) out[row * dim + d] = float_to_elem<DT>(some ? o / L : 0.0f);
             if (out_acc) out_acc[row * dim + d] = o;
             if (xo.world && out_acc) xchg_put(xo, xepoch, xchg_word_index(xo, row, d), __float_as_uint(o));
         }
         // (the host only asks for a fan-out of 16-bit outputs when the vector path above is taken)
     }
     if (tid == 0) {
-        if (out_lse) out_lse[row] = L > 0.0f ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
+        if (out_lse) out_lse[row] = some ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
         if (out_ml) { out_ml[row * 2] = M; out_ml[row * 2 + 1] = L; }
         if (xo.world && out_ml) xchg_put2(xo, xepoch, xo.rank_off + xo_ml_off + row * 2, __float_as_uint(M), __float_as_uint(L));
     }
@@ -584,7 +586,7 @@ __global__ void __launch_bounds__(kCombineThreads)
 lse_combine_kernel(const float* __restrict__ part_acc, int64_t acc_ps, int64_t acc_rs,
                    const float* __restrict__ part_ml, int64_t ml_ps, int64_t ml_rs, int n_part, int dim,
                    uint16_t* __restrict__ out, float* __restrict__ out_lse, float* __restrict__ out_acc,
-                   float* __restrict__ out_ml, const XchgLL ll, int64_t ll_ml_off, const XchgOut xo, int64_t xo_ml_off) {
+                   float* __restrict__ out_ml, const XchgLL ll, int64_t ll_ml_off, const XchgOut xo, int64_t xo_ml_off, bool keep_nan) {
     pdl_launch_dependents();
     pdl_wait();
     // results that other ranks need go straight into every rank's exchange buffer as well (pair format):
@@ -592,7 +594,7 @@ lse_combine_kernel(const float* __restrict__ part_acc, int64_t acc_ps, int64_t a
     const uint32_t xepoch = xo.world ? xchg_next_epoch(xo) : 0u;
     const uint32_t want = ll.chan != nullptr ? ll.epoch[ll.channel] : 0u;
     combine_row<DT>(part_acc, acc_ps, acc_rs, part_ml, ml_ps, ml_rs, n_part, dim, out, out_lse, out_acc, out_ml, ll,
-                    ll_ml_off, want, xo, xo_ml_off, xepoch);
+                    ll_ml_off, want, xo, xo_ml_off, xepoch, keep_nan);
     if (xo.world) xchg_finish(xo, xepoch, gridDim.x);
 }
 
@@ -606,18 +608,18 @@ __global__ void __launch_bounds__(kCombineThreads)
 lse_combine_exchange_kernel(const float* __restrict__ part_acc, int64_t acc_ps, int64_t acc_rs,
                             const float* __restrict__ part_ml, int64_t ml_ps, int64_t ml_rs, int n_part, int dim,
                             float* __restrict__ out_acc, float* __restrict__ out_ml, const XchgOut xo, int64_t ml_off,
-                            const XchgLL ll, uint16_t* __restrict__ out, float* __restrict__ out_lse) {
+                            const XchgLL ll, uint16_t* __restrict__ out, float* __restrict__ out_lse, bool keep_nan) {
     pdl_launch_dependents();
     pdl_wait();
     const uint32_t xepoch = xchg_next_epoch(xo);
     const XchgLL none = {};
     combine_row<DT>(part_acc, acc_ps, acc_rs, part_ml, ml_ps, ml_rs, n_part, dim, nullptr, nullptr, out_acc, out_ml, none,
-                    0, 0u, xo, ml_off, xepoch);
+                    0, 0u, xo, ml_off, xepoch, keep_nan);
     xchg_finish(xo, xepoch, gridDim.x);   // starts with a block barrier: the shared arrays are free again
     XchgOut off = xo;
     off.world = 0;
     combine_row<DT>(nullptr, 0, 0, nullptr, 0, 0, ll.world, dim, out, out_lse, nullptr, nullptr, ll, ml_off, xepoch, off, 0,
-                    0u);
+                    0u, keep_nan);
 }
 
 template <int DT, int LPR>
@@ -645,13 +647,13 @@ __global__ void __launch_bounds__(kCombineThreads)
 lse_combine_allgather_kernel(const float* __restrict__ part_acc, int64_t acc_ps, int64_t acc_rs,
                              const float* __restrict__ part_ml, int64_t ml_ps, int64_t ml_rs, int n_part, int dim,
                              uint16_t* __restrict__ out, float* __restrict__ out_lse, const XchgOut xo, const XchgLL ll,
-                             uint32_t* __restrict__ dense) {
+                             uint32_t* __restrict__ dense, bool keep_nan) {
     pdl_launch_dependents();
     pdl_wait();
     const uint32_t xepoch = xchg_next_epoch(xo);
     const XchgLL none = {};
     combine_row<DT>(part_acc, acc_ps, acc_rs, part_ml, ml_ps, ml_rs, n_part, dim, out, out_lse, nullptr, nullptr, none, 0,
-                    0u, xo, 0, xepoch);
+                    0u, xo, 0, xepoch, keep_nan);
     xchg_finish(xo, xepoch, gridDim.x);
     // words of row (b, h) of rank r: block b, rank offset r * slice, row h of the slice (the layout of xo)
     const int64_t row = blockIdx.x;
@@ -708,7 +710,7 @@ int64_t attend_scratch_bytes(int n_prob, int group, int head_dim) {
 
 int lse_combine(const float* acc, int64_t acc_ps, int64_t acc_rs, const float* ml, int64_t ml_ps, int64_t ml_rs,
                 int n_part, int64_t rows, int head_dim, int dtype, void* out, float* out_lse, float* out_acc,
-                float* out_ml, cudaStream_t stream, const XchgLL* ll, const XchgOut* xout, const XchgFinal* fin) {
+                float* out_ml, cudaStream_t stream, const XchgLL* ll, const XchgOut* xout, const XchgFinal* fin, bool keep_nan) {
     // fin (may be NULL; needs xout and out_acc / out_ml): after the fan-out the same launch waits for the other
     // ranks' blocks and writes the merge of all ranks' parts to fin->out
     // ll (may be NULL): the parts arrive in pair format in an exchange channel instead of acc / ml
@@ -736,11 +738,11 @@ int lse_combine(const float* acc, int64_t acc_ps, int64_t acc_rs, const float* m
         if (dtype == DC_BF16)
             DC_CUDA_TRY(launch_chained(lse_combine_allgather_kernel<DC_BF16>, grid, block, 0, stream, 0u, acc, acc_ps, acc_rs,
                                        ml, ml_ps, ml_rs, n_part, head_dim, static_cast<uint16_t*>(out), out_lse, xo, fin->ll,
-                                       static_cast<uint32_t*>(fin->out)));
+                                       static_cast<uint32_t*>(fin->out), keep_nan));
         else
             DC_CUDA_TRY(launch_chained(lse_combine_allgather_kernel<DC_FP16>, grid, block, 0, stream, 0u, acc, acc_ps, acc_rs,
                                        ml, ml_ps, ml_rs, n_part, head_dim, static_cast<uint16_t*>(out), out_lse, xo, fin->ll,
-                                       static_cast<uint32_t*>(fin->out)));
+                                       static_cast<uint32_t*>(fin->out), keep_nan));
         return DC_OK;
     }
     if (fin != nullptr) {
@@ -752,21 +754,21 @@ int lse_combine(const float* acc, int64_t acc_ps, int64_t acc_rs, const float* m
         if (dtype == DC_BF16)
             DC_CUDA_TRY(launch_chained(lse_combine_exchange_kernel<DC_BF16>, grid, block, 0, stream, 0u, acc, acc_ps, acc_rs,
                                        ml, ml_ps, ml_rs, n_part, head_dim, out_acc, out_ml, xo, ml_off, fin->ll,
-                                       static_cast<uint16_t*>(fin->out), fin->out_lse));
+                                       static_cast<uint16_t*>(fin->out), fin->out_lse, keep_nan));
         else
             DC_CUDA_TRY(launch_chained(lse_combine_exchange_kernel<DC_FP16>, grid, block, 0, stream, 0u, acc, acc_ps, acc_rs,
                                        ml, ml_ps, ml_rs, n_part, head_dim, out_acc, out_ml, xo, ml_off, fin->ll,
-                                       static_cast<uint16_t*>(fin->out), fin->out_lse));
+                                       static_cast<uint16_t*>(fin->out), fin->out_lse, keep_nan));
         return DC_OK;
     }
     if (dtype == DC_BF16)
         DC_CUDA_TRY(launch_chained(lse_combine_kernel<DC_BF16>, grid, block, 0, stream, 0u, acc, acc_ps, acc_rs, ml, ml_ps,
                                    ml_rs, n_part, head_dim, static_cast<uint16_t*>(out), out_lse, out_acc, out_ml, w, ml_off,
-                                   xo, ml_off));
+                                   xo, ml_off, keep_nan));
     else
         DC_CUDA_TRY(launch_chained(lse_combine_kernel<DC_FP16>, grid, block, 0, stream, 0u, acc, acc_ps, acc_rs, ml, ml_ps,
                                    ml_rs, n_part, head_dim, static_cast<uint16_t*>(out), out_lse, out_acc, out_ml, w, ml_off,
-                                   xo, ml_off));
+                                   xo, ml_off, keep_nan));
     return DC_OK;
 }
 
@@ -847,7 +849,7 @@ int sparse_attend(const void* k_store, const void* v_store, int64_t prob_stride,
     if (rc != DC_OK) return rc;
     return lse_combine(a.part_acc, head_dim, static_cast<int64_t>(a.n_split) * head_dim, a.part_ml, 2,
                        static_cast<int64_t>(a.n_split) * 2, a.n_split, static_cast<int64_t>(n_prob) * group, head_dim,
-                       dtype, out, out_lse, out_acc, out_ml, stream, nullptr, xout, fin);
+                       dtype, out, out_lse, out_acc, out_ml, stream, nullptr, xout, fin, false);
 }
 
 }  // namespace dc

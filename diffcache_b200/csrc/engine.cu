@@ -9,10 +9,12 @@
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
+#include <new>
 #include <string>
 #include <vector>
 
 #include "exchange.cuh"
+#include "q4.cuh"
 
 namespace dc {
 
@@ -42,7 +44,7 @@ int64_t attend_scratch_bytes(int n_prob, int group, int head_dim);
 int lse_combine(const float* acc, int64_t acc_ps, int64_t acc_rs, const float* ml, int64_t ml_ps, int64_t ml_rs,
                 int n_part, int64_t rows, int head_dim, int dtype, void* out, float* out_lse, float* out_acc,
                 float* out_ml, cudaStream_t stream, const XchgLL* ll = nullptr, const XchgOut* xout = nullptr,
-                const XchgFinal* fin = nullptr);
+                const XchgFinal* fin = nullptr, bool keep_nan = false);
 int pq_build_lut(const void* q, int q_mode, int group, int dtype, const float* centroids, int n_prob, int head_dim,
                  int n_sub, float* lut, cudaStream_t stream);
 int pq_adc_scan(const uint8_t* codes, int64_t prob_stride, int n_prob, int64_t n, int n_sub, const float* lut,
@@ -225,6 +227,26 @@ __global__ void window_advance_kernel(int32_t* win) {
     }
 }
 
+// out[p][i] = row ids[p][i], or row row0 + i, of a 16-bit store; rows outside the stored ones are zeros
+__global__ void read_rows_kernel(const uint16_t* __restrict__ k_store, const uint16_t* __restrict__ v_store,
+                                 int64_t prob_stride, int dim, const int32_t* __restrict__ len,
+                                 const uint32_t* __restrict__ ids, int64_t row0, int64_t n, uint16_t* __restrict__ out_k,
+                                 uint16_t* __restrict__ out_v) {
+    const int lanes = dim / 8;
+    const int64_t prob = blockIdx.y;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * (blockDim.x / lanes) + threadIdx.x / lanes;
+    const int c = threadIdx.x % lanes;
+    if (i >= n) return;
+    const int64_t row = ids != nullptr ? static_cast<int64_t>(ids[prob * n + i]) : row0 + i;
+    const int64_t src = prob * prob_stride + row * dim + c * 8, dst = (prob * n + i) * dim + c * 8;
+    const bool ok = row < len[0];
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    if (out_k) *reinterpret_cast<uint4*>(out_k + dst) = ok ? *reinterpret_cast<const uint4*>(k_store + src) : zero;
+    if (out_v) *reinterpret_cast<uint4*>(out_v + dst) = ok ? *reinterpret_cast<const uint4*>(v_store + src) : zero;
+}
+
+__global__ void raise_len_kernel(int32_t* len, int32_t value) { len[0] = max(len[0], value); }
+
 bool is_device_ptr(const void* p) {
     if (p == nullptr) return true;
     cudaPointerAttributes at;
@@ -257,8 +279,10 @@ struct dc_engine {
     void* out_dense = nullptr;         // dc_set_output_gather: where the step's last kernel unpacks all ranks' slices
     int64_t prob_stride = 0;   // elements
     int64_t score_stride = 0;  // elements
-    uint16_t* k = nullptr;
+    uint16_t* k = nullptr;     // 16-bit store (NULL in a 4-bit engine)
     uint16_t* v = nullptr;
+    bool q4 = false;           // rows are held in 4 bits (q4.cuh), in `st`
+    Q4Store st = {};
     uint32_t* scores = nullptr;
     uint32_t* minmax = nullptr;
     uint32_t* sel_idx = nullptr;   // (n_prob, DC_MAX_TOPK) worst case, used with stride = k
@@ -357,8 +381,10 @@ int scan_and_select(dc_engine* e, const void* q, int q_mode, int k, int64_t n_bo
     // e->minmax is in its initial state here: set once in dc_create, and put back by every select
     if (ev) DC_CUDA_TRY(cudaEventRecord(ev[0], s));
     trace_mark(e, s);
-    int rc = score_scan(e->k, e->prob_stride, e->n_prob, n_bound, e->head_dim, e->dtype, q, q_mode, e->group, e->scores,
-                        e->score_stride, e->minmax, s, e->status, e->kv_heads, q_stride_b, e->len);
+    int rc = e->q4 ? q4_score_scan(e->st.k, e->st.prob_rows, e->n_prob, n_bound, e->head_dim, e->dtype, q, q_mode, e->group,
+                                   e->scores, e->score_stride, e->minmax, s, e->kv_heads, q_stride_b, e->len)
+                   : score_scan(e->k, e->prob_stride, e->n_prob, n_bound, e->head_dim, e->dtype, q, q_mode, e->group,
+                                e->scores, e->score_stride, e->minmax, s, e->status, e->kv_heads, q_stride_b, e->len);
     if (rc) return rc;
     if (ev) DC_CUDA_TRY(cudaEventRecord(ev[1], s));
     trace_mark(e, s);
@@ -399,6 +425,73 @@ int copy_rows_in(dc_engine* e, const void* src, uint16_t* store, int64_t seq_len
     return DC_OK;
 }
 
+// keys / vals -> rows [row0, row0 + n) of a 4-bit store.  Host sources go through a bounded staging buffer, one
+// problem and at most 65536 rows at a time; the call then returns synchronised.
+int q4_rows_in(dc_engine* e, const void* keys, const void* vals, int64_t n, int64_t row0, int64_t stride_b,
+               int64_t stride_h, int64_t stride_s, int len_mode, cudaStream_t s) {
+    if (is_device_ptr(keys) && is_device_ptr(vals))
+        return q4_write_rows(keys, vals, stride_b, stride_h, stride_s, e->n_prob, e->kv_heads, n, e->head_dim, e->dtype,
+                             e->st, row0, e->len, len_mode, s);
+    const int64_t D = e->head_dim, piece = std::min<int64_t>(n, 65536);
+    const size_t es = sizeof(uint16_t);
+    uint16_t* stage = nullptr;
+    int rc = DC_OK;
+    if (n > 0) DC_CUDA_TRY(cudaMalloc(reinterpret_cast<void**>(&stage), 2 * piece * D * es));
+    for (int p = 0; p < e->n_prob && rc == DC_OK; p++) {
+        const int64_t off = (p / e->kv_heads) * stride_b + (p % e->kv_heads) * stride_h;
+        Q4Store st = e->st;   // this problem's rows
+        for (Q4Rows* t : {&st.k, &st.v}) {
+            t->codes += p * st.prob_rows * q4_code_bytes(e->head_dim);
+            t->scales += p * st.prob_rows * (D / kQ4Group);
+        }
+        for (int64_t i = 0; i < n && rc == DC_OK; i += piece) {
+            const int64_t m = std::min(piece, n - i);
+            cudaError_t err = cudaSuccess;
+            for (int which = 0; which < 2 && err == cudaSuccess; which++)
+                err = cudaMemcpy2DAsync(stage + which * piece * D, D * es,
+                                        static_cast<const uint16_t*>(which ? vals : keys) + off + i * stride_s, stride_s * es,
+                                        D * es, m, cudaMemcpyDefault, s);
+            if (err != cudaSuccess) rc = cuda_fail(err, "copy of host rows");
+            else rc = q4_write_rows(stage, stage + piece * D, 0, 0, D, 1, 1, m, e->head_dim, e->dtype, st, row0 + i,
+                                    nullptr, kLenKeep, s);
+        }
+    }
+    if (rc == DC_OK && len_mode == kLenSet) set_len_kernel<<<1, 1, 0, s>>>(e->len, static_cast<int32_t>(row0 + n));
+    if (rc == DC_OK && len_mode == kLenMax) raise_len_kernel<<<1, 1, 0, s>>>(e->len, static_cast<int32_t>(row0 + n));
+    cudaError_t err = cudaGetLastError();
+    if (err == cudaSuccess) err = cudaStreamSynchronize(s);
+    cudaFree(stage);
+    return rc == DC_OK && err != cudaSuccess ? cuda_fail(err, "write of host rows") : rc;
+}
+
+// The attention of a step over this engine's store, whichever format it has (arguments as in sparse_attend).
+int attend_store(dc_engine* e, int64_t bound, const void* q, int64_t q_stride_b, const uint32_t* sel, int n_sel,
+                 int64_t sel_base, const int32_t* sel_count, const int32_t* lens, const void* k_new, const void* v_new,
+                 int64_t new_stride_b, void* res_k, void* res_v, int64_t res_stride_b, int64_t res_stride_h, int res_len,
+                 const int32_t* res_len_dev, float scale, void* out, float* out_lse, float* out_acc, float* out_ml,
+                 const XchgOut* xout, const XchgFinal* fin, cudaStream_t s) {
+    if (!e->q4)
+        return sparse_attend(e->k, e->v, e->prob_stride, bound, e->n_prob, e->kv_heads, e->group, e->head_dim, e->dtype,
+                             q, sel, n_sel, n_sel, sel_base, k_new, v_new, res_k, res_v, res_stride_b, res_stride_h, res_len,
+                             scale, out, out_lse, out_acc, out_ml, e->att_scratch, s, sel_count, q_stride_b, new_stride_b,
+                             e->len, res_len_dev, xout, fin);
+    Q4Attend a = {};
+    a.st = e->st;
+    a.n_rows = bound; a.n_rows_dev = e->len;
+    a.n_prob = e->n_prob; a.kv_heads = e->kv_heads; a.group = e->group; a.head_dim = e->head_dim; a.dtype = e->dtype;
+    a.q = q; a.q_stride_b = q_stride_b;
+    a.sel = sel; a.sel_stride = n_sel; a.n_sel = n_sel; a.sel_base = sel_base; a.sel_count = sel_count;
+    a.lens = lens;
+    a.k_new = k_new; a.v_new = v_new; a.new_stride_b = new_stride_b;
+    a.res_k = res_k; a.res_v = res_v; a.res_stride_b = res_stride_b; a.res_stride_h = res_stride_h;
+    a.res_len = res_len; a.res_len_dev = res_len_dev;
+    a.scale = scale;
+    a.out = out; a.out_lse = out_lse; a.out_acc = out_acc; a.out_ml = out_ml;
+    a.scratch = e->att_scratch;
+    a.xout = xout; a.fin = fin;
+    return q4_attend(a, s);
+}
+
 int decode_attend_impl(dc_engine* e, const void* q, int64_t q_stride_b, const void* k_new, const void* v_new,
                        int64_t new_stride_b, void* res_k, void* res_v, int64_t res_stride_b, int64_t res_stride_h,
                        int res_len, const int32_t* res_len_dev, int topk, float scale, void* out, int32_t* out_idx,
@@ -424,8 +517,8 @@ const char* dc_last_error(void) { return g_err; }
 
 int dc_version(void) { return 100; }
 
-int dc_create(int bsz, int q_heads, int kv_heads, int head_dim, int64_t max_ctx_len, int dtype, int device,
-              dc_engine** out) {
+static int create_engine(int bsz, int q_heads, int kv_heads, int head_dim, int64_t max_ctx_len, int dtype, int device,
+                         bool q4, dc_engine** out) {
     DC_REQUIRE(out != nullptr, "dc_create: null out");
     *out = nullptr;
     DC_REQUIRE(bsz >= 1 && kv_heads >= 1 && q_heads >= 1, "dc_create: bsz/q_heads/kv_heads must be positive");
@@ -439,7 +532,9 @@ int dc_create(int bsz, int q_heads, int kv_heads, int head_dim, int64_t max_ctx_
     DeviceGuard guard(device);
     if (!guard.ok) { set_error("dc_create: cannot select device %d", device); return DC_ECUDA; }
 
-    dc_engine* e = new dc_engine();
+    dc_engine* e = new (std::nothrow) dc_engine();
+    if (e == nullptr) { set_error("dc_create: out of host memory"); return DC_ENOMEM; }
+    e->q4 = q4;
     e->bsz = bsz; e->q_heads = q_heads; e->kv_heads = kv_heads; e->head_dim = head_dim; e->dtype = dtype;
     e->device = device; e->n_prob = bsz * kv_heads; e->group = q_heads / kv_heads;
     e->max_ctx = max_ctx_len;
@@ -450,8 +545,18 @@ int dc_create(int bsz, int q_heads, int kv_heads, int head_dim, int64_t max_ctx_
     auto alloc = [&](void** p, size_t bytes) {
         if (err == cudaSuccess) err = cudaMalloc(p, std::max<size_t>(bytes, 256));
     };
-    alloc(reinterpret_cast<void**>(&e->k), store_bytes);
-    alloc(reinterpret_cast<void**>(&e->v), store_bytes);
+    const size_t rows_total = static_cast<size_t>(e->n_prob) * max_ctx_len;
+    const size_t code_bytes = rows_total * q4_code_bytes(head_dim), scale_bytes = rows_total * q4_scale_bytes(head_dim);
+    if (q4) {
+        e->st.prob_rows = max_ctx_len;
+        for (Q4Rows* t : {&e->st.k, &e->st.v}) {
+            alloc(reinterpret_cast<void**>(&t->codes), code_bytes);
+            alloc(reinterpret_cast<void**>(&t->scales), scale_bytes);
+        }
+    } else {
+        alloc(reinterpret_cast<void**>(&e->k), store_bytes);
+        alloc(reinterpret_cast<void**>(&e->v), store_bytes);
+    }
     alloc(reinterpret_cast<void**>(&e->scores), static_cast<size_t>(e->n_prob) * e->score_stride * sizeof(uint32_t));
     alloc(reinterpret_cast<void**>(&e->minmax), static_cast<size_t>(e->n_prob) * 2 * sizeof(uint32_t));
     const size_t sel_cap = static_cast<size_t>(std::min<int64_t>(DC_MAX_TOPK, max_ctx_len));
@@ -459,14 +564,22 @@ int dc_create(int bsz, int q_heads, int kv_heads, int head_dim, int64_t max_ctx_
     alloc(reinterpret_cast<void**>(&e->sel_bits), static_cast<size_t>(e->n_prob) * sel_cap * sizeof(uint32_t));
     alloc(reinterpret_cast<void**>(&e->status), 256);
     alloc(reinterpret_cast<void**>(&e->budget), static_cast<size_t>(e->n_prob) * sizeof(int32_t));
-    alloc(&e->att_scratch, static_cast<size_t>(attend_scratch_bytes(e->n_prob, e->group, head_dim)));
+    alloc(&e->att_scratch, static_cast<size_t>(q4 ? q4_attend_scratch_bytes(e->n_prob, e->group, head_dim)
+                                                  : attend_scratch_bytes(e->n_prob, e->group, head_dim)));
     alloc(reinterpret_cast<void**>(&e->q_dev), static_cast<size_t>(bsz) * q_heads * head_dim * sizeof(uint16_t));
     alloc(reinterpret_cast<void**>(&e->len), 256);
     alloc(reinterpret_cast<void**>(&e->ins_stage), 2 * static_cast<size_t>(e->n_prob) * head_dim * sizeof(uint16_t));
     if (err == cudaSuccess) err = cudaMemset(e->len, 0, 256);
     if (err == cudaSuccess) err = cudaMemset(e->status, 0, 256);
-    if (err == cudaSuccess) err = cudaMemset(e->k, 0, store_bytes);   // the reference zero-fills its store
-    if (err == cudaSuccess) err = cudaMemset(e->v, 0, store_bytes);   // (HugeArray, diffcache_cpu/src/lib.rs:91-105)
+    if (!q4) {
+        if (err == cudaSuccess) err = cudaMemset(e->k, 0, store_bytes);   // the reference zero-fills its store
+        if (err == cudaSuccess) err = cudaMemset(e->v, 0, store_bytes);   // (HugeArray, diffcache_cpu/src/lib.rs:91-105)
+    } else {
+        for (Q4Rows* t : {&e->st.k, &e->st.v}) {   // scale 0: every row reads as zeros
+            if (err == cudaSuccess) err = cudaMemset(t->codes, 0x88, code_bytes);
+            if (err == cudaSuccess) err = cudaMemset(t->scales, 0, scale_bytes);
+        }
+    }
     if (err != cudaSuccess) {
         int rc = cuda_fail(err, "dc_create allocation");
         dc_destroy(e);
@@ -480,10 +593,23 @@ int dc_create(int bsz, int q_heads, int kv_heads, int head_dim, int64_t max_ctx_
     return DC_OK;
 }
 
+int dc_create(int bsz, int q_heads, int kv_heads, int head_dim, int64_t max_ctx_len, int dtype, int device,
+              dc_engine** out) {
+    return create_engine(bsz, q_heads, kv_heads, head_dim, max_ctx_len, dtype, device, false, out);
+}
+
+int dc_create_q4(int bsz, int q_heads, int kv_heads, int head_dim, int64_t max_ctx_len, int dtype, int device,
+                 dc_engine** out) {
+    return create_engine(bsz, q_heads, kv_heads, head_dim, max_ctx_len, dtype, device, true, out);
+}
+
+int dc_store_bits(dc_engine* e) { return e == nullptr ? 0 : e->q4 ? 4 : 16; }
+
 int dc_destroy(dc_engine* e) {
     if (e == nullptr) return DC_OK;
     DeviceGuard guard(e->device);
     cudaDeviceSynchronize();
+    cudaFree(e->st.k.codes); cudaFree(e->st.k.scales); cudaFree(e->st.v.codes); cudaFree(e->st.v.scales);
     cudaFree(e->k); cudaFree(e->v); cudaFree(e->scores); cudaFree(e->minmax); cudaFree(e->sel_idx);
     cudaFree(e->sel_bits); cudaFree(e->status); cudaFree(e->budget); cudaFree(e->att_scratch); cudaFree(e->q_dev);
     cudaFree(e->stage_k); cudaFree(e->stage_v); cudaFree(e->len); cudaFree(e->ins_stage);
@@ -512,12 +638,16 @@ int dc_prefill(dc_engine* e, const void* keys, const void* vals, int64_t seq_len
                    ((reinterpret_cast<uintptr_t>(keys) | reinterpret_cast<uintptr_t>(vals)) & 15) == 0,
                "dc_prefill: pointers must be 16-byte aligned and strides multiples of 8 elements");
     cudaStream_t s = as_stream(stream);
-    int rc = copy_rows_in(e, keys, e->k, seq_len, 0, stride_b, stride_h, stride_s, s);
+    int rc = e->q4 ? q4_rows_in(e, keys, vals, seq_len, 0, stride_b, stride_h, stride_s, kLenSet, s) : DC_OK;
     if (rc) return rc;
-    rc = copy_rows_in(e, vals, e->v, seq_len, 0, stride_b, stride_h, stride_s, s);
-    if (rc) return rc;
-    set_len_kernel<<<1, 1, 0, s>>>(e->len, static_cast<int32_t>(seq_len));
-    DC_CUDA_TRY(cudaGetLastError());
+    if (!e->q4) {
+        rc = copy_rows_in(e, keys, e->k, seq_len, 0, stride_b, stride_h, stride_s, s);
+        if (rc) return rc;
+        rc = copy_rows_in(e, vals, e->v, seq_len, 0, stride_b, stride_h, stride_s, s);
+        if (rc) return rc;
+        set_len_kernel<<<1, 1, 0, s>>>(e->len, static_cast<int32_t>(seq_len));
+        DC_CUDA_TRY(cudaGetLastError());
+    }
     e->ctx_len = seq_len;
     e->len_on_device = false;
     if (!is_device_ptr(keys) || !is_device_ptr(vals)) DC_CUDA_TRY(cudaStreamSynchronize(s));
@@ -547,9 +677,14 @@ int dc_insert(dc_engine* e, const void* keys, const void* vals, uint64_t stream)
     }
     DC_REQUIRE(((reinterpret_cast<uintptr_t>(kd) | reinterpret_cast<uintptr_t>(vd)) & 15) == 0,
                "dc_insert: keys/vals must be 16-byte aligned");
-    append_rows_kernel<<<1, 1024, 0, s>>>(kd, vd, e->n_prob, e->head_dim, e->k, e->v, e->prob_stride, e->max_ctx, e->len,
-                                          e->status);
-    DC_CUDA_TRY(cudaGetLastError());
+    if (e->q4) {
+        int rc = q4_append_rows(kd, vd, e->n_prob, e->head_dim, e->dtype, e->st, e->max_ctx, e->len, e->status, s);
+        if (rc) return rc;
+    } else {
+        append_rows_kernel<<<1, 1024, 0, s>>>(kd, vd, e->n_prob, e->head_dim, e->k, e->v, e->prob_stride, e->max_ctx, e->len,
+                                              e->status);
+        DC_CUDA_TRY(cudaGetLastError());
+    }
     if (e->ctx_len < e->max_ctx) e->ctx_len += 1;
     if (host_src) DC_CUDA_TRY(cudaStreamSynchronize(s));
     return DC_OK;
@@ -604,13 +739,15 @@ int dc_query(dc_engine* e, const void* q_mean, int ef, void* out_keys, void* out
     }
     if (out_keys) {
         void* dst = k_host ? static_cast<void*>(e->stage_k) : out_keys;
-        rc = gather_rows(e->k, e->prob_stride, e->n_prob, D, e->sel_idx, k, k, dst, s);
+        rc = e->q4 ? q4_read_rows(e->st, ctx, e->len, e->n_prob, D, e->dtype, 0, e->sel_idx, k, k, dst, nullptr, false, s)
+                   : gather_rows(e->k, e->prob_stride, e->n_prob, D, e->sel_idx, k, k, dst, s);
         if (rc) return rc;
         if (k_host) { host_io = true; DC_CUDA_TRY(cudaMemcpyAsync(out_keys, dst, rows * D * es, cudaMemcpyDeviceToHost, s)); }
     }
     if (out_vals) {
         void* dst = v_host ? static_cast<void*>(e->stage_v) : out_vals;
-        rc = gather_rows(e->v, e->prob_stride, e->n_prob, D, e->sel_idx, k, k, dst, s);
+        rc = e->q4 ? q4_read_rows(e->st, ctx, e->len, e->n_prob, D, e->dtype, 0, e->sel_idx, k, k, nullptr, dst, false, s)
+                   : gather_rows(e->v, e->prob_stride, e->n_prob, D, e->sel_idx, k, k, dst, s);
         if (rc) return rc;
         if (v_host) { host_io = true; DC_CUDA_TRY(cudaMemcpyAsync(out_vals, dst, rows * D * es, cudaMemcpyDeviceToHost, s)); }
     }
@@ -636,6 +773,13 @@ int dc_get_keys(dc_engine* e, float* out) {
     const size_t per_prob = static_cast<size_t>(ctx) * e->head_dim;
     auto convert = [&](int p0, int np, float* dst) {
         dim3 grid(256, np);
+        if (e->q4) {
+            Q4Store st = e->st;
+            st.k.codes += static_cast<int64_t>(p0) * st.prob_rows * q4_code_bytes(e->head_dim);
+            st.k.scales += static_cast<int64_t>(p0) * st.prob_rows * (e->head_dim / kQ4Group);
+            q4_read_rows(st, ctx, nullptr, np, e->head_dim, e->dtype, 0, nullptr, 0, ctx, dst, nullptr, true, nullptr);
+            return cudaGetLastError();
+        }
         const uint16_t* src = e->k + static_cast<int64_t>(p0) * e->prob_stride;
         if (e->dtype == DC_BF16) keys_to_f32_kernel<DC_BF16><<<grid, 256>>>(src, e->prob_stride, ctx, e->head_dim, dst);
         else keys_to_f32_kernel<DC_FP16><<<grid, 256>>>(src, e->prob_stride, ctx, e->head_dim, dst);
@@ -666,6 +810,10 @@ int dc_get_keys(dc_engine* e, float* out) {
 int dc_export_rows(dc_engine* e, void* keys_out, void* vals_out) {
     DC_ENGINE_ENTER(e);
     DC_REQUIRE(keys_out && vals_out, "dc_export_rows: null pointer");
+    if (e->q4) {
+        set_error("dc_export_rows: the rows are held in 4 bits (dc_export_q4 copies them, dc_read_rows reads them back)");
+        return DC_ESTATE;
+    }
     int64_t ctx = 0;
     int rc = host_ctx_len(e, nullptr, &ctx);
     if (rc) return rc;
@@ -676,6 +824,158 @@ int dc_export_rows(dc_engine* e, void* keys_out, void* vals_out) {
     DC_CUDA_TRY(cudaMemcpy2D(vals_out, row_bytes, e->v, e->prob_stride * sizeof(uint16_t), row_bytes, e->n_prob,
                              cudaMemcpyDefault));
     return DC_OK;
+}
+
+// which = 0: store -> caller, 1: caller -> store; rows [0, n) of every problem
+static int copy_q4(dc_engine* e, void* const ptr[4], int64_t n, int into) {
+    const Q4Rows* t[2] = {&e->st.k, &e->st.v};
+    for (int i = 0; i < 4 && n > 0; i++) {
+        const size_t row = i & 1 ? q4_scale_bytes(e->head_dim) : q4_code_bytes(e->head_dim);
+        void* mine = i & 1 ? static_cast<void*>(t[i / 2]->scales) : static_cast<void*>(t[i / 2]->codes);
+        const size_t pitch = static_cast<size_t>(e->max_ctx) * row, width = static_cast<size_t>(n) * row;
+        if (into) DC_CUDA_TRY(cudaMemcpy2D(mine, pitch, ptr[i], width, width, e->n_prob, cudaMemcpyDefault));
+        else DC_CUDA_TRY(cudaMemcpy2D(ptr[i], width, mine, pitch, width, e->n_prob, cudaMemcpyDefault));
+    }
+    return DC_OK;
+}
+
+int dc_export_q4(dc_engine* e, void* k_codes, void* k_scales, void* v_codes, void* v_scales) {
+    DC_ENGINE_ENTER(e);
+    DC_REQUIRE(k_codes && k_scales && v_codes && v_scales, "dc_export_q4: null pointer");
+    if (!e->q4) { set_error("dc_export_q4: the rows are held in 16 bits (dc_export_rows)"); return DC_ESTATE; }
+    int64_t ctx = 0;
+    int rc = host_ctx_len(e, nullptr, &ctx);
+    if (rc) return rc;
+    DC_CUDA_TRY(cudaDeviceSynchronize());
+    void* const ptr[4] = {k_codes, k_scales, v_codes, v_scales};
+    return copy_q4(e, ptr, ctx, 0);
+}
+
+int dc_import_q4(dc_engine* e, const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,
+                 int64_t n) {
+    DC_ENGINE_ENTER(e);
+    DC_REQUIRE(k_codes && k_scales && v_codes && v_scales, "dc_import_q4: null pointer");
+    DC_REQUIRE(n >= 0 && n <= e->max_ctx, "dc_import_q4: n=%lld exceeds max_ctx_len=%lld", static_cast<long long>(n),
+               static_cast<long long>(e->max_ctx));
+    if (!e->q4) { set_error("dc_import_q4: the rows are held in 16 bits (dc_prefill)"); return DC_ESTATE; }
+    DC_CUDA_TRY(cudaDeviceSynchronize());
+    void* const ptr[4] = {const_cast<void*>(k_codes), const_cast<void*>(k_scales), const_cast<void*>(v_codes),
+                          const_cast<void*>(v_scales)};
+    int rc = copy_q4(e, ptr, n, 1);
+    if (rc) return rc;
+    set_len_kernel<<<1, 1>>>(e->len, static_cast<int32_t>(n));
+    DC_CUDA_TRY(cudaGetLastError());
+    DC_CUDA_TRY(cudaDeviceSynchronize());
+    e->ctx_len = n;
+    e->len_on_device = false;
+    return DC_OK;
+}
+
+int dc_write_rows(dc_engine* e, const void* keys, const void* vals, int64_t row0, int64_t n, int64_t stride_b,
+                  int64_t stride_h, int64_t stride_s, uint64_t stream) {
+    DC_ENGINE_ENTER(e);
+    DC_REQUIRE(n >= 0 && row0 >= 0 && n <= e->max_ctx && row0 <= e->max_ctx - n,
+               "dc_write_rows: rows [%lld, %lld + %lld) exceed max_ctx_len=%lld", static_cast<long long>(row0),
+               static_cast<long long>(row0), static_cast<long long>(n), static_cast<long long>(e->max_ctx));
+    if (e->len_on_device) {
+        set_error("dc_write_rows: after dc_window_push only the device knows where the stored rows end");
+        return DC_ESTATE;
+    }
+    DC_REQUIRE(row0 <= e->ctx_len, "dc_write_rows: row0=%lld leaves a gap behind the %lld stored rows",
+               static_cast<long long>(row0), static_cast<long long>(e->ctx_len));
+    if (n == 0) return DC_OK;
+    DC_REQUIRE(keys && vals, "dc_write_rows: null keys/vals");
+    DC_REQUIRE(stride_b >= 0 && stride_h >= 0 && stride_s >= 0 && stride_b % 8 == 0 && stride_h % 8 == 0 && stride_s % 8 == 0 &&
+                   ((reinterpret_cast<uintptr_t>(keys) | reinterpret_cast<uintptr_t>(vals)) & 15) == 0,
+               "dc_write_rows: pointers must be 16-byte aligned and strides non-negative multiples of 8 elements");
+    cudaStream_t s = as_stream(stream);
+    int rc = DC_OK;
+    if (e->q4) {
+        rc = q4_rows_in(e, keys, vals, n, row0, stride_b, stride_h, stride_s, kLenMax, s);
+        if (rc) return rc;
+    } else {
+        rc = copy_rows_in(e, keys, e->k, n, row0, stride_b, stride_h, stride_s, s);
+        if (rc == DC_OK) rc = copy_rows_in(e, vals, e->v, n, row0, stride_b, stride_h, stride_s, s);
+        if (rc) return rc;
+        raise_len_kernel<<<1, 1, 0, s>>>(e->len, static_cast<int32_t>(row0 + n));
+        DC_CUDA_TRY(cudaGetLastError());
+        if (!is_device_ptr(keys) || !is_device_ptr(vals)) DC_CUDA_TRY(cudaStreamSynchronize(s));
+    }
+    e->ctx_len = std::max(e->ctx_len, row0 + n);
+    return DC_OK;
+}
+
+int dc_read_rows(dc_engine* e, int64_t row0, const uint32_t* ids, int64_t n, void* out_keys, void* out_vals, uint64_t stream) {
+    DC_ENGINE_ENTER(e);
+    DC_REQUIRE(n >= 0 && row0 >= 0 && n < (1ll << 31), "dc_read_rows: row0=%lld n=%lld", static_cast<long long>(row0),
+               static_cast<long long>(n));
+    DC_REQUIRE(ids != nullptr || row0 + n <= e->max_ctx, "dc_read_rows: rows [%lld, %lld + %lld) exceed max_ctx_len=%lld",
+               static_cast<long long>(row0), static_cast<long long>(row0), static_cast<long long>(n),
+               static_cast<long long>(e->max_ctx));
+    if (n == 0 || (out_keys == nullptr && out_vals == nullptr)) return DC_OK;
+    DC_REQUIRE(is_device_ptr(ids) && is_device_ptr(out_keys) && is_device_ptr(out_vals), "dc_read_rows: device pointers only");
+    DC_REQUIRE(((reinterpret_cast<uintptr_t>(out_keys) | reinterpret_cast<uintptr_t>(out_vals)) & 15) == 0 &&
+                   (reinterpret_cast<uintptr_t>(ids) & 3) == 0,
+               "dc_read_rows: outputs must be 16-byte aligned");
+    cudaStream_t s = as_stream(stream);
+    if (e->q4)
+        return q4_read_rows(e->st, e->max_ctx, e->len, e->n_prob, e->head_dim, e->dtype, row0, ids, n, n, out_keys, out_vals,
+                            false, s);
+    const int64_t rpb = 256 / (e->head_dim / 8);
+    read_rows_kernel<<<dim3(static_cast<unsigned>((n + rpb - 1) / rpb), e->n_prob), 256, 0, s>>>(
+        e->k, e->v, e->prob_stride, e->head_dim, e->len, ids, row0, n, static_cast<uint16_t*>(out_keys),
+        static_cast<uint16_t*>(out_vals));
+    DC_CUDA_TRY(cudaGetLastError());
+    return DC_OK;
+}
+
+int dc_score_rows(dc_engine* e, const void* q, int q_mode, int64_t n, uint32_t* out_bits, int64_t out_stride, uint64_t stream) {
+    DC_ENGINE_ENTER(e);
+    DC_REQUIRE(q && out_bits, "dc_score_rows: null pointer");
+    DC_REQUIRE(q_mode == 0 || q_mode == 1, "dc_score_rows: q_mode=%d", q_mode);
+    DC_REQUIRE(n >= 0 && n <= e->max_ctx && out_stride >= n, "dc_score_rows: n=%lld out_stride=%lld max_ctx_len=%lld",
+               static_cast<long long>(n), static_cast<long long>(out_stride), static_cast<long long>(e->max_ctx));
+    DC_REQUIRE((reinterpret_cast<uintptr_t>(q) & 15) == 0 && (reinterpret_cast<uintptr_t>(out_bits) & 3) == 0,
+               "dc_score_rows: q must be 16-byte aligned");
+    DC_REQUIRE(is_device_ptr(q) && is_device_ptr(out_bits), "dc_score_rows: device pointers only");
+    cudaStream_t s = as_stream(stream);
+    if (e->q4)   // the kernel clamps n to the rows stored when it runs
+        return q4_score_scan(e->st.k, e->st.prob_rows, e->n_prob, n, e->head_dim, e->dtype, q, q_mode, e->group, out_bits,
+                             out_stride, nullptr, s, e->kv_heads, 0, e->len);
+    int64_t ctx = 0;
+    int rc = host_ctx_len(e, s, &ctx);
+    if (rc) return rc;
+    return score_scan(e->k, e->prob_stride, e->n_prob, std::min(n, ctx), e->head_dim, e->dtype, q, q_mode, e->group, out_bits,
+                      out_stride, nullptr, s, e->status, e->kv_heads, 0, nullptr);
+}
+
+int dc_attend_rows(dc_engine* e, const void* q, int64_t q_stride_b, const uint32_t* ids, int n_ids, const int32_t* lens,
+                   const void* k_new, const void* v_new, int64_t new_stride_b, void* res_k, void* res_v,
+                   int64_t res_stride_b, int64_t res_stride_h, int res_len, float scale, void* out, float* out_lse,
+                   uint64_t stream) {
+    DC_ENGINE_ENTER(e);
+    DC_REQUIRE(q && out, "dc_attend_rows: null q/out");
+    DC_REQUIRE(n_ids >= 0 || ids == nullptr, "dc_attend_rows: ids given with n_ids < 0");
+    DC_REQUIRE(lens == nullptr || n_ids < 0, "dc_attend_rows: lens only limits attention over all rows (n_ids < 0)");
+    DC_REQUIRE(q_stride_b >= 0 && new_stride_b >= 0 && q_stride_b % 8 == 0 && new_stride_b % 8 == 0,
+               "dc_attend_rows: batch strides must be non-negative multiples of 8 elements");
+    DC_REQUIRE(q_stride_b == 0 || q_stride_b >= static_cast<int64_t>(e->q_heads) * e->head_dim,
+               "dc_attend_rows: q batch stride smaller than one batch of query heads");
+    DC_REQUIRE(new_stride_b == 0 || new_stride_b >= static_cast<int64_t>(e->kv_heads) * e->head_dim,
+               "dc_attend_rows: k_new/v_new batch stride smaller than one batch of kv heads");
+    DC_REQUIRE(is_device_ptr(q) && is_device_ptr(ids) && is_device_ptr(lens) && is_device_ptr(out) && is_device_ptr(k_new) &&
+                   is_device_ptr(v_new) && is_device_ptr(res_k) && is_device_ptr(res_v) && is_device_ptr(out_lse),
+               "dc_attend_rows: device pointers only");
+    if (n_ids < 0 && !e->q4) {
+        set_error("dc_attend_rows: attention over every stored row needs a 4-bit store (dc_create_q4)");
+        return DC_ESTATE;
+    }
+    int64_t bound = 0;
+    int rc = rows_bound(e, as_stream(stream), &bound);
+    if (rc) return rc;
+    return attend_store(e, bound, q, q_stride_b, ids, n_ids, 0, nullptr, lens, k_new, v_new, new_stride_b, res_k, res_v,
+                        res_stride_b, res_stride_h, res_len, nullptr, scale, out, out_lse, nullptr, nullptr, nullptr,
+                        nullptr, as_stream(stream));
 }
 
 int dc_update_r_sq(dc_engine* e, const float* r_sq, int n) {
@@ -761,10 +1061,8 @@ int decode_attend_impl(dc_engine* e, const void* q, int64_t q_stride_b, const vo
             finp = &fin;
         }
     }
-    rc = sparse_attend(e->k, e->v, e->prob_stride, bound, e->n_prob, e->kv_heads, e->group, e->head_dim, e->dtype,
-                       q, e->sel_idx, k, k, 0, k_new, v_new, res_k, res_v, res_stride_b, res_stride_h, res_len, scale,
-                       out, out_lse, nullptr, nullptr, e->att_scratch, s, sel_count, q_stride_b, new_stride_b, e->len,
-                       res_len_dev, xout, finp);
+    rc = attend_store(e, bound, q, q_stride_b, e->sel_idx, k, 0, sel_count, nullptr, k_new, v_new, new_stride_b, res_k, res_v,
+                      res_stride_b, res_stride_h, res_len, res_len_dev, scale, out, out_lse, nullptr, nullptr, xout, finp, s);
     if (rc) return rc;
     if (ev) {
         DC_CUDA_TRY(cudaEventRecord(ev[3], s));
@@ -793,6 +1091,9 @@ int dc_window_push(dc_engine* e, const void* k_new, const void* v_new, int64_t n
                "dc_window_push: device pointers only");
     cudaStream_t s = as_stream(stream);
     e->len_on_device = true;  // from here on only the device knows how many rows the store holds
+    if (e->q4)
+        return q4_window_push(k_new, v_new, new_stride_b, res_k, res_v, res_stride_b, res_stride_h, e->n_prob, e->kv_heads,
+                              e->head_dim, e->dtype, e->st, e->max_ctx, e->len, window_state, e->status, s);
     DC_CUDA_TRY(launch_chained(window_push_kernel, dim3(1), dim3(1024), 0, s, 0u, static_cast<const uint16_t*>(k_new),
                                static_cast<const uint16_t*>(v_new), new_stride_b, static_cast<uint16_t*>(res_k),
                                static_cast<uint16_t*>(res_v), res_stride_b, res_stride_h, e->n_prob, e->kv_heads,
@@ -954,10 +1255,10 @@ static int attend_owned_impl(dc_engine* e, const void* q, const uint32_t* sel_gi
     int64_t bound = 0;
     int rc = rows_bound(e, as_stream(stream), &bound);
     if (rc) return rc;
-    return sparse_attend(e->k, e->v, e->prob_stride, bound, e->n_prob, e->kv_heads, e->group, e->head_dim,
-                         e->dtype, q, sel_gidx, n_sel, n_sel, e->row_offset, k_new, v_new, res_k, res_v, res_stride_b,
-                         res_stride_h, res_len, scale, nullptr, nullptr, out_acc, out_ml, e->att_scratch,
-                         as_stream(stream), sel_count, 0, 0, e->len, nullptr, xout, fin);
+    DC_REQUIRE(n_sel >= 0, "dc_attend_owned: negative n_sel");
+    return attend_store(e, bound, q, 0, sel_gidx, n_sel, e->row_offset, sel_count, nullptr, k_new, v_new, 0, res_k, res_v,
+                        res_stride_b, res_stride_h, res_len, nullptr, scale, nullptr, nullptr, out_acc, out_ml, xout, fin,
+                        as_stream(stream));
 }
 
 // ---- sequence-sharded step with the two exchanges done by peer stores (exchange.cu) ----
@@ -1092,7 +1393,7 @@ int dc_sharded_combine(dc_engine* e, dc_xchg* x, void* out, float* out_lse, uint
     const int64_t rows = static_cast<int64_t>(e->n_prob) * e->group;
     const XchgLL w1 = xchg_ll_args(x, 1);
     int rc = lse_combine(nullptr, 0, 0, nullptr, 0, 0, xchg_world(x), rows, e->head_dim, e->dtype, out, out_lse, nullptr,
-                         nullptr, as_stream(stream), &w1);
+                         nullptr, as_stream(stream), &w1, nullptr, nullptr, e->q4);
     if (rc) return rc;
     return trace_mark(e, as_stream(stream));
 }
@@ -1119,6 +1420,100 @@ int dc_sharded_decode_attend(dc_engine* e, dc_xchg* x, const void* q, const void
     rc = dc_sharded_attend(e, x, q, k_new, v_new, res_k, res_v, res_stride_b, res_stride_h, res_len, scale, stream);
     if (rc) return rc;
     return dc_sharded_combine(e, x, out, out_lse, stream);
+}
+
+// ---- 4-bit rows, stateless ----
+
+static int q4_store_checked(const char* who, const void* k_codes, const void* k_scales, const void* v_codes,
+                            const void* v_scales, int64_t prob_rows, int n_prob, int head_dim, int dtype, Q4Store* out) {
+    DC_REQUIRE(dtype == DC_BF16 || dtype == DC_FP16, "%s: dtype %d not supported", who, dtype);
+    DC_REQUIRE(head_dim == 64 || head_dim == 128 || head_dim == 256, "%s: head_dim %d not in {64,128,256}", who, head_dim);
+    DC_REQUIRE(n_prob >= 0 && n_prob <= 65535 && prob_rows >= 0 && prob_rows < (1ll << 31), "%s: n_prob=%d prob_rows=%lld", who,
+               n_prob, static_cast<long long>(prob_rows));
+    DC_REQUIRE(((reinterpret_cast<uintptr_t>(k_codes) | reinterpret_cast<uintptr_t>(v_codes) |
+                 reinterpret_cast<uintptr_t>(k_scales) | reinterpret_cast<uintptr_t>(v_scales)) & 15) == 0,
+               "%s: codes and scales must be 16-byte aligned", who);
+    out->k.codes = static_cast<uint8_t*>(const_cast<void*>(k_codes));
+    out->k.scales = static_cast<uint16_t*>(const_cast<void*>(k_scales));
+    out->v.codes = static_cast<uint8_t*>(const_cast<void*>(v_codes));
+    out->v.scales = static_cast<uint16_t*>(const_cast<void*>(v_scales));
+    out->prob_rows = prob_rows;
+    return DC_OK;
+}
+
+int dc_q4_write_rows(const void* keys, const void* vals, int64_t stride_b, int64_t stride_h, int64_t stride_s, int n_prob,
+                     int kv_heads, int64_t n, int head_dim, int dtype, void* k_codes, void* k_scales, void* v_codes,
+                     void* v_scales, int64_t prob_rows, int64_t row0, uint64_t stream) {
+    DC_REQUIRE(keys && vals && k_codes && k_scales && v_codes && v_scales, "dc_q4_write_rows: null pointer");
+    Q4Store st;
+    int rc = q4_store_checked("dc_q4_write_rows", k_codes, k_scales, v_codes, v_scales, prob_rows, n_prob, head_dim, dtype, &st);
+    if (rc) return rc;
+    DC_REQUIRE(kv_heads >= 1 && n >= 0 && row0 >= 0 && n <= prob_rows && row0 <= prob_rows - n,
+               "dc_q4_write_rows: kv_heads=%d, rows [%lld, %lld + %lld) of %lld", kv_heads, static_cast<long long>(row0),
+               static_cast<long long>(row0), static_cast<long long>(n), static_cast<long long>(prob_rows));
+    DC_REQUIRE(stride_b >= 0 && stride_h >= 0 && stride_s >= 0 && stride_b % 8 == 0 && stride_h % 8 == 0 && stride_s % 8 == 0 &&
+                   ((reinterpret_cast<uintptr_t>(keys) | reinterpret_cast<uintptr_t>(vals)) & 15) == 0,
+               "dc_q4_write_rows: keys/vals must be 16-byte aligned and strides non-negative multiples of 8 elements");
+    return q4_write_rows(keys, vals, stride_b, stride_h, stride_s, n_prob, kv_heads, n, head_dim, dtype, st, row0, nullptr,
+                         kLenKeep, as_stream(stream));
+}
+
+int dc_q4_read_rows(const void* codes, const void* scales, int64_t prob_rows, int64_t n_rows, int n_prob, int head_dim,
+                    int dtype, int64_t row0, const uint32_t* ids, int64_t ids_stride, int64_t n, void* out, uint64_t stream) {
+    DC_REQUIRE(codes && scales && out, "dc_q4_read_rows: null pointer");
+    Q4Store st;
+    int rc = q4_store_checked("dc_q4_read_rows", codes, scales, codes, scales, prob_rows, n_prob, head_dim, dtype, &st);
+    if (rc) return rc;
+    DC_REQUIRE(n_rows >= 0 && n_rows <= prob_rows && n >= 0 && n < (1ll << 31) && row0 >= 0 && (ids == nullptr || ids_stride >= n),
+               "dc_q4_read_rows: n_rows=%lld n=%lld row0=%lld ids_stride=%lld", static_cast<long long>(n_rows),
+               static_cast<long long>(n), static_cast<long long>(row0), static_cast<long long>(ids_stride));
+    DC_REQUIRE((reinterpret_cast<uintptr_t>(out) & 15) == 0, "dc_q4_read_rows: out must be 16-byte aligned");
+    return q4_read_rows(st, n_rows, nullptr, n_prob, head_dim, dtype, row0, ids, ids_stride, n, out, nullptr, false,
+                        as_stream(stream));
+}
+
+int dc_q4_score_scan(const void* codes, const void* scales, int64_t prob_rows, int n_prob, int64_t n, int head_dim, int dtype,
+                     const void* q, int q_mode, int group, uint32_t* scores, int64_t score_stride, uint32_t* minmax,
+                     uint64_t stream) {
+    DC_REQUIRE(codes && scales && q && scores, "dc_q4_score_scan: null pointer");
+    Q4Store st;
+    int rc = q4_store_checked("dc_q4_score_scan", codes, scales, codes, scales, prob_rows, n_prob, head_dim, dtype, &st);
+    if (rc) return rc;
+    DC_REQUIRE(n >= 0 && n <= prob_rows && score_stride >= n, "dc_q4_score_scan: n=%lld prob_rows=%lld score_stride=%lld",
+               static_cast<long long>(n), static_cast<long long>(prob_rows), static_cast<long long>(score_stride));
+    DC_REQUIRE(q_mode == 0 || (q_mode == 1 && group >= 1), "dc_q4_score_scan: bad q_mode/group");
+    DC_REQUIRE((reinterpret_cast<uintptr_t>(q) & 15) == 0, "dc_q4_score_scan: q must be 16-byte aligned");
+    return q4_score_scan(st.k, prob_rows, n_prob, n, head_dim, dtype, q, q_mode, group, scores, score_stride, minmax,
+                         as_stream(stream));
+}
+
+int64_t dc_q4_attend_scratch_bytes(int n_prob, int group, int head_dim) {
+    return q4_attend_scratch_bytes(n_prob, group, head_dim);
+}
+
+int dc_q4_attend(const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales, int64_t prob_rows,
+                 int64_t n_rows, int n_prob, int kv_heads, int group, int head_dim, int dtype, const void* q,
+                 const uint32_t* sel, int64_t sel_stride, int n_sel, int64_t sel_base, const int32_t* lens, const void* k_new,
+                 const void* v_new, void* res_k, void* res_v, int64_t res_stride_b, int64_t res_stride_h, int res_len,
+                 float scale, void* out, float* out_lse, float* out_acc, float* out_ml, void* scratch, uint64_t stream) {
+    Q4Attend a = {};
+    int rc = q4_store_checked("dc_q4_attend", k_codes, k_scales, v_codes, v_scales, prob_rows, n_prob, head_dim, dtype, &a.st);
+    if (rc) return rc;
+    DC_REQUIRE(n_rows >= 0 && n_rows <= prob_rows, "dc_q4_attend: n_rows=%lld prob_rows=%lld", static_cast<long long>(n_rows),
+               static_cast<long long>(prob_rows));
+    DC_REQUIRE(n_rows == 0 || n_sel == 0 || (k_codes && k_scales && v_codes && v_scales), "dc_q4_attend: null store");
+    DC_REQUIRE(lens == nullptr || n_sel < 0, "dc_q4_attend: lens only limits attention over all rows (n_sel < 0)");
+    a.n_rows = n_rows;
+    a.n_prob = n_prob; a.kv_heads = kv_heads; a.group = group; a.head_dim = head_dim; a.dtype = dtype;
+    a.q = q;
+    a.sel = sel; a.sel_stride = sel_stride; a.n_sel = n_sel; a.sel_base = sel_base;
+    a.lens = lens;
+    a.k_new = k_new; a.v_new = v_new;
+    a.res_k = res_k; a.res_v = res_v; a.res_stride_b = res_stride_b; a.res_stride_h = res_stride_h; a.res_len = res_len;
+    a.scale = scale;
+    a.out = out; a.out_lse = out_lse; a.out_acc = out_acc; a.out_ml = out_ml;
+    a.scratch = scratch;
+    return q4_attend(a, as_stream(stream));
 }
 
 // ---- stateless kernels ----

@@ -1,0 +1,246 @@
+// Rows into and out of a store held in 4 bits (format: q4.cuh).
+//
+// Counterpart of copy_rows / append / gather on the 16-bit store: DataLayer::prefill and insert
+// (diffcache_cpu/src/lib.rs:329-369, nsw.rs:497-557) and the row gather of search_bruteforce (nsw.rs:621-629),
+// which the reference does with plain copies.
+//
+// A thread holds 8 consecutive elements (one 16-byte load); the group maximum is two shuffles, the codes move to
+// their stored order with two more, and the row leaves as 4-byte words that the head_dim / 8 threads of a row write
+// side by side.  Bound: HBM (2 * head_dim bytes in, 9/16 * head_dim out per row, or the other way round).
+#include "q4.cuh"
+
+namespace dc {
+namespace {
+
+constexpr int kRowThreads = 256;
+
+struct WriteArgs {
+    const uint16_t* src[2];     // keys, values
+    int64_t stride_b, stride_h, stride_s;
+    int kv_heads;
+    int64_t n, row0;
+    Q4Store st;
+    int32_t* len;
+    int len_mode;
+};
+
+template <int D>
+__device__ __forceinline__ void q4_put(const Q4Rows& t, int64_t row, int v, uint32_t word, uint16_t scale) {
+    reinterpret_cast<uint32_t*>(t.codes + row * (D / 2))[q4_word_index<D>(v)] = word;
+    if ((v & 3) == 0) t.scales[row * (D / kQ4Group) + (v >> 2)] = scale;
+}
+
+// grid = (row blocks, n_prob, 2 tensors)
+template <int DT, int D>
+__global__ void __launch_bounds__(kRowThreads)
+q4_write_kernel(const WriteArgs a) {
+    pdl_launch_dependents();
+    pdl_wait();
+    constexpr int LPR = D / 8, RPB = kRowThreads / LPR;
+    const int64_t prob = blockIdx.y;
+    const int v = threadIdx.x % LPR;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * RPB + threadIdx.x / LPR;
+    const bool ok = i < a.n;
+    const int64_t b = prob / a.kv_heads, h = prob % a.kv_heads;
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (ok) w = ld_stream16(a.src[blockIdx.z] + b * a.stride_b + h * a.stride_h + i * a.stride_s + v * 8);
+    uint16_t scale;
+    const uint32_t word = q4_encode8<DT>(w, v, scale);
+    if (ok) q4_put<D>(blockIdx.z ? a.st.v : a.st.k, prob * a.st.prob_rows + a.row0 + i, v, word, scale);
+    if (a.len_mode != kLenKeep && blockIdx.x == 0 && prob == 0 && blockIdx.z == 0 && threadIdx.x == 0) {
+        const int32_t end = static_cast<int32_t>(a.row0 + a.n);
+        a.len[0] = a.len_mode == kLenSet ? end : max(a.len[0], end);
+    }
+}
+
+// Index::insert (diffcache_cpu/src/nsw.rs:544-557): row len[0] of every problem <- keys / vals (n_prob, D), then
+// len[0] += 1.  One CTA, so that every thread sees the old length.
+template <int DT, int D>
+__global__ void __launch_bounds__(1024)
+q4_append_kernel(const uint16_t* __restrict__ keys, const uint16_t* __restrict__ vals, int n_prob, const Q4Store st,
+                 int64_t max_rows, int32_t* len, uint32_t* status) {
+    constexpr int LPR = D / 8;
+    const int64_t n = len[0];
+    if (n >= max_rows) {   // full: nothing is written (the host-side call reports it when it can tell)
+        if (threadIdx.x == 0 && status) atomicMax(status, 301u);
+        return;
+    }
+    const int total = n_prob * 2 * LPR;
+    for (int i0 = 0; i0 < total; i0 += blockDim.x) {   // all lanes of a warp stay in the loop: the encoder shuffles
+        const int i = i0 + threadIdx.x;
+        const bool ok = i < total;
+        const int p = i / (2 * LPR), which = (i / LPR) & 1, v = i % LPR;
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (ok) w = *reinterpret_cast<const uint4*>((which ? vals : keys) + static_cast<int64_t>(p) * D + v * 8);
+        uint16_t scale;
+        const uint32_t word = q4_encode8<DT>(w, v, scale);
+        if (ok) q4_put<D>(which ? st.v : st.k, p * st.prob_rows + n, v, word, scale);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) len[0] = static_cast<int32_t>(n + 1);
+}
+
+// The window ring of the resident buffer (see window_push_kernel in engine.cu: same state words, same statuses) with the
+// spilled token quantised on its way into the store.
+template <int DT, int D>
+__global__ void __launch_bounds__(1024)
+q4_window_push_kernel(const uint16_t* __restrict__ k_new, const uint16_t* __restrict__ v_new, int64_t new_stride_b,
+                      uint16_t* __restrict__ res_k, uint16_t* __restrict__ res_v, int64_t res_stride_b,
+                      int64_t res_stride_h, int n_prob, int kv_heads, const Q4Store st, int64_t max_rows, int32_t* len,
+                      int32_t* win, uint32_t* status) {
+    pdl_launch_dependents();
+    pdl_wait();
+    constexpr int LPR = D / 8;
+    const int suffix_len = win[0], head = win[1], prefix_len = win[2], cap = win[3];
+    const int64_t n = len[0];
+    const bool full = suffix_len >= cap;
+    const bool spill = full && n < max_rows;
+    const int slot = full ? head : suffix_len;
+    if (full && !spill && threadIdx.x == 0 && status) atomicMax(status, 302u);  // store full: the oldest token is dropped
+    const int total = n_prob * 2 * LPR;
+    for (int i0 = 0; i0 < total; i0 += blockDim.x) {
+        const int i = i0 + threadIdx.x;
+        const bool ok = i < total;
+        const int p = i / (2 * LPR), which = (i / LPR) & 1, v = i % LPR;
+        const int b = p / kv_heads, h = p % kv_heads;
+        uint16_t* row = (which ? res_v : res_k) + b * res_stride_b + h * res_stride_h +
+                        static_cast<int64_t>(prefix_len + slot) * D + v * 8;
+        if (spill) {
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (ok) w = *reinterpret_cast<const uint4*>(row);
+            uint16_t scale;
+            const uint32_t word = q4_encode8<DT>(w, v, scale);
+            if (ok) q4_put<D>(which ? st.v : st.k, p * st.prob_rows + n, v, word, scale);
+        }
+        const int64_t off = new_stride_b ? b * new_stride_b + static_cast<int64_t>(h) * D : static_cast<int64_t>(p) * D;
+        if (ok) *reinterpret_cast<uint4*>(row) = *reinterpret_cast<const uint4*>((which ? v_new : k_new) + off + v * 8);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        if (spill) len[0] = static_cast<int32_t>(n + 1);
+        win[4] = prefix_len + min(suffix_len + 1, cap);
+    }
+}
+
+struct ReadArgs {
+    Q4Store st;
+    int64_t n_rows;
+    const int32_t* n_dev;
+    const uint32_t* ids;        // (n_prob, ids_stride) or NULL: rows row0, row0 + 1, ...
+    int64_t ids_stride, row0, n;
+    void* out[2];
+};
+
+// grid = (row blocks, n_prob, outputs)
+template <int DT, int D, bool F32>
+__global__ void __launch_bounds__(kRowThreads)
+q4_read_kernel(const ReadArgs a) {
+    pdl_launch_dependents();
+    pdl_wait();
+    constexpr int LPR = D / 8, RPB = kRowThreads / LPR;
+    const int64_t prob = blockIdx.y;
+    const int v = threadIdx.x % LPR;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * RPB + threadIdx.x / LPR;
+    const int which = a.out[0] == nullptr ? 1 : blockIdx.z;
+    const int64_t n_rows = a.n_dev != nullptr ? static_cast<int64_t>(*a.n_dev) : a.n_rows;
+    uint32_t word = 0x88888888u;
+    uint16_t scale = 0;
+    if (i < a.n) {
+        const int64_t row = a.ids != nullptr ? static_cast<int64_t>(a.ids[prob * a.ids_stride + i]) : a.row0 + i;
+        if (row < n_rows) {   // a pad (0xFFFFFFFF) or any id beyond the stored rows reads as zeros
+            const Q4Rows& t = which ? a.st.v : a.st.k;
+            const int64_t r = prob * a.st.prob_rows + row;
+            word = __ldcs(reinterpret_cast<const uint32_t*>(t.codes + r * (D / 2)) + q4_word_index<D>(v));
+            scale = t.scales[r * (D / kQ4Group) + (v >> 2)];
+        }
+    }
+    if (F32) {
+        word = q4_transpose_in(word, v);
+        if (i >= a.n) return;
+        const float s = elem_to_float<DT>(scale);
+        float* o = static_cast<float*>(a.out[which]) + (prob * a.n + i) * D + v * 8;
+#pragma unroll
+        for (int e = 0; e < 8; e++) o[e] = static_cast<float>(static_cast<int>((word >> (4 * e)) & 15u) - 8) * s;
+    } else {
+        const uint4 w = q4_decode8<DT>(word, scale, v);
+        if (i < a.n) __stcs(reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out[which]) + (prob * a.n + i) * D + v * 8), w);
+    }
+}
+
+}  // namespace
+
+#define DC_Q4_DISPATCH(dtype, head_dim, CASE)                 \
+    if ((dtype) == DC_BF16) {                                 \
+        if ((head_dim) == 64) { CASE(DC_BF16, 64); }          \
+        else if ((head_dim) == 128) { CASE(DC_BF16, 128); }   \
+        else { CASE(DC_BF16, 256); }                          \
+    } else {                                                  \
+        if ((head_dim) == 64) { CASE(DC_FP16, 64); }          \
+        else if ((head_dim) == 128) { CASE(DC_FP16, 128); }   \
+        else { CASE(DC_FP16, 256); }                          \
+    }
+
+int q4_write_rows(const void* keys, const void* vals, int64_t stride_b, int64_t stride_h, int64_t stride_s, int n_prob,
+                  int kv_heads, int64_t n, int head_dim, int dtype, const Q4Store& st, int64_t row0, int32_t* len,
+                  int len_mode, cudaStream_t stream) {
+    if (n_prob == 0 || (n == 0 && len_mode == kLenKeep)) return DC_OK;
+    WriteArgs a;
+    a.src[0] = static_cast<const uint16_t*>(keys);
+    a.src[1] = static_cast<const uint16_t*>(vals);
+    a.stride_b = stride_b; a.stride_h = stride_h; a.stride_s = stride_s;
+    a.kv_heads = kv_heads;
+    a.n = n; a.row0 = row0;
+    a.st = st;
+    a.len = len; a.len_mode = len_mode;
+    const int64_t rpb = kRowThreads / (head_dim / 8);
+    const dim3 grid(static_cast<unsigned>(n > 0 ? (n + rpb - 1) / rpb : 1), static_cast<unsigned>(n_prob), 2u);
+#define CASE(DT, D) DC_CUDA_TRY(launch_chained(q4_write_kernel<DT, D>, grid, dim3(kRowThreads), 0, stream, 0u, a))
+    DC_Q4_DISPATCH(dtype, head_dim, CASE)
+#undef CASE
+    return DC_OK;
+}
+
+int q4_append_rows(const void* keys, const void* vals, int n_prob, int head_dim, int dtype, const Q4Store& st,
+                   int64_t max_rows, int32_t* len, uint32_t* status, cudaStream_t stream) {
+    const uint16_t* k = static_cast<const uint16_t*>(keys);
+    const uint16_t* v = static_cast<const uint16_t*>(vals);
+#define CASE(DT, D) q4_append_kernel<DT, D><<<1, 1024, 0, stream>>>(k, v, n_prob, st, max_rows, len, status)
+    DC_Q4_DISPATCH(dtype, head_dim, CASE)
+#undef CASE
+    DC_CUDA_TRY(cudaGetLastError());
+    return DC_OK;
+}
+
+int q4_window_push(const void* k_new, const void* v_new, int64_t new_stride_b, void* res_k, void* res_v,
+                   int64_t res_stride_b, int64_t res_stride_h, int n_prob, int kv_heads, int head_dim, int dtype,
+                   const Q4Store& st, int64_t max_rows, int32_t* len, int32_t* win, uint32_t* status, cudaStream_t stream) {
+#define CASE(DT, D)                                                                                                     \
+    DC_CUDA_TRY(launch_chained(q4_window_push_kernel<DT, D>, dim3(1), dim3(1024), 0, stream, 0u,                        \
+                               static_cast<const uint16_t*>(k_new), static_cast<const uint16_t*>(v_new), new_stride_b, \
+                               static_cast<uint16_t*>(res_k), static_cast<uint16_t*>(res_v), res_stride_b, res_stride_h, \
+                               n_prob, kv_heads, st, max_rows, len, win, status))
+    DC_Q4_DISPATCH(dtype, head_dim, CASE)
+#undef CASE
+    return DC_OK;
+}
+
+int q4_read_rows(const Q4Store& st, int64_t n_rows, const int32_t* n_dev, int n_prob, int head_dim, int dtype, int64_t row0,
+                 const uint32_t* ids, int64_t ids_stride, int64_t n, void* out_k, void* out_v, bool f32, cudaStream_t stream) {
+    if (n_prob == 0 || n == 0 || (out_k == nullptr && out_v == nullptr)) return DC_OK;
+    ReadArgs a;
+    a.st = st;
+    a.n_rows = n_rows; a.n_dev = n_dev;
+    a.ids = ids; a.ids_stride = ids_stride;
+    a.row0 = row0; a.n = n;
+    a.out[0] = out_k; a.out[1] = out_v;
+    const int64_t rpb = kRowThreads / (head_dim / 8);
+    const dim3 grid(static_cast<unsigned>((n + rpb - 1) / rpb), static_cast<unsigned>(n_prob), out_k && out_v ? 2u : 1u);
+#define CASE(DT, D)                                                                                             \
+    if (f32) DC_CUDA_TRY(launch_chained(q4_read_kernel<DT, D, true>, grid, dim3(kRowThreads), 0, stream, 0u, a)); \
+    else DC_CUDA_TRY(launch_chained(q4_read_kernel<DT, D, false>, grid, dim3(kRowThreads), 0, stream, 0u, a))
+    DC_Q4_DISPATCH(dtype, head_dim, CASE)
+#undef CASE
+    return DC_OK;
+}
+
+}  // namespace dc

@@ -102,17 +102,24 @@ class DiffCacheGPU:
     scan, i.e. the reference's ``use_bruteforce=True`` semantics.  Two keyword-only
     additions select the element type and device: ``dtype`` ("bf16" | "fp16") and
     ``device`` (CUDA ordinal); ``adaptive_budget=True`` applies the reference's k-check
-    (``k_check_seq``, ``attn_mass_threshold``) to the fused step."""
+    (``k_check_seq``, ``attn_mass_threshold``) to the fused step.  ``store_bits=4`` holds the
+    rows in 4 bits (groups of 32 elements with one scale, see ``dc_create_q4``): every method
+    works on the rows as they are read back, the store is 3.56 times smaller and the scan reads
+    that much less."""
 
     def __init__(self, bsz: int, q_head_num: int, kv_head_num: int, head_dim: int, **kwargs):
         dtype = kwargs.pop("dtype", "bf16")
         device = kwargs.pop("device", None)
+        store_bits = kwargs.pop("store_bits", 16)
         adaptive = bool(kwargs.pop("adaptive_budget", False))
         opts = dict(_OPTION_DEFAULTS)
         for key, value in kwargs.items():
             if key not in opts:
                 raise ValueError(f"Unknown option {key}")
             opts[key] = value
+        if store_bits not in (4, 16):
+            raise ValueError(f"store_bits must be 4 or 16, got {store_bits}")
+        self.store_bits = int(store_bits)
         if opts["r_sq"] is None:
             opts["r_sq"] = [4.0] * kv_head_num
         self.options = opts
@@ -127,8 +134,9 @@ class DiffCacheGPU:
         self.metrics = _metric_names(self.name)
         self._lib = _lib.load()
         handle = ctypes.c_void_p()
-        _lib.check(self._lib.dc_create(bsz, q_head_num, kv_head_num, head_dim, int(opts["max_ctx_len"]), self.dtype,
-                                       self.device, ctypes.byref(handle)))
+        create = self._lib.dc_create_q4 if self.store_bits == 4 else self._lib.dc_create
+        _lib.check(create(bsz, q_head_num, kv_head_num, head_dim, int(opts["max_ctx_len"]), self.dtype,
+                          self.device, ctypes.byref(handle)))
         self._h = handle
         if adaptive:
             self.set_adaptive_budget(opts["k_check_seq"], opts["attn_mass_threshold"])
@@ -260,6 +268,152 @@ class DiffCacheGPU:
         from . import snapshot
 
         snapshot.load_engine(self, path, ctx_len)
+
+    # -- stored rows -------------------------------------------------------------------------
+    def write_rows(self, row0: int, keys, vals, stream=None) -> None:
+        """Writes (or overwrites) stored rows ``[row0, row0 + n)``, e.g. one chunk of a chunked prefill;
+        ``keys``/``vals`` ``(bsz, kv_head_num, n, head_dim)`` as in :meth:`prefill`.  ``row0`` may be at most
+        ``ctx_len``; the store then holds ``max(ctx_len, row0 + n)`` rows."""
+        shape = (self.bsz, self.kv_head_num, None, self.head_dim)
+        n = self._check(keys, shape, "keys")[2]
+        self._check(vals, (self.bsz, self.kv_head_num, n, self.head_dim), "vals")
+        sk, sv = self._row_strides(keys, "keys"), self._row_strides(vals, "vals")
+        if sk != sv:
+            raise ValueError("keys and vals must share one stride pattern")
+        _lib.check(self._lib.dc_write_rows(self._h, _ptr(keys), _ptr(vals), int(row0), n, *sk, self._stream(stream)))
+
+    def read_rows(self, out_keys, out_vals, row0: int = 0, ids=None, stream=None) -> None:
+        """Reads stored rows back into ``out_keys``/``out_vals`` ``(bsz, kv_head_num, n, head_dim)`` (dense device
+        tensors of the element type; ``None`` skips one): rows ``row0 ..``, or the rows ``ids`` ``(bsz,
+        kv_head_num, n)`` int32.  Rows that are not stored (negative ids, positions beyond ``ctx_len``) are zeros."""
+        n = None
+        for x, what in ((out_keys, "out_keys"), (out_vals, "out_vals")):
+            if x is not None:
+                n = self._check(x, (self.bsz, self.kv_head_num, n, self.head_dim), what, device_only=True, dense=True)[2]
+        if n is None:
+            return
+        if ids is not None:
+            self._check_words(ids, (self.bsz, self.kv_head_num, n), "ids")
+        _lib.check(self._lib.dc_read_rows(self._h, int(row0), _ptr(ids), n, _ptr(out_keys), _ptr(out_vals),
+                                          self._stream(stream)))
+
+    def score_rows(self, q, out_bits, stream=None) -> None:
+        """Ranking keys ``bits(65536 - <q, k>)`` of the first ``n`` stored rows into ``out_bits`` ``(bsz, kv_head_num,
+        n)`` (32-bit device tensor; entries beyond the stored rows stay as they are).  ``q`` ``(bsz, kv_head_num,
+        head_dim)`` holds one (group-mean) vector per kv head, or ``(bsz, q_head_num, head_dim)`` the query
+        heads, whose group mean is taken."""
+        heads = _shape(q)[1] if len(_shape(q)) == 3 else -1
+        mode = 0 if heads == self.kv_head_num else 1
+        self._check(q, (self.bsz, self.kv_head_num if mode == 0 else self.q_head_num, self.head_dim), "q", device_only=True,
+                    dense=True)
+        n = self._check_words(out_bits, (self.bsz, self.kv_head_num, None), "out_bits")[2]
+        _lib.check(self._lib.dc_score_rows(self._h, _ptr(q), mode, n, _ptr(out_bits), n, self._stream(stream)))
+
+    def attend_rows(self, q, out, ids=None, lens=None, res_k=None, res_v=None, res_len: int = 0, k_new=None, v_new=None,
+                    scale: float = 0.0, out_lse=None, stream=None) -> None:
+        """Softmax attention of every query head over the stored rows ``ids`` ``(bsz, kv_head_num, k)`` int32 (ids that
+        are not stored are skipped), the resident rows and the new token; arguments as in :meth:`decode_attend`.
+        Without ``ids`` (4-bit stores): every stored row, of sequence ``b`` only the first ``lens[b]`` (int32
+        device tensor ``(bsz,)``) when ``lens`` is given.  Heads that have nothing to attend over get 0, and -inf in
+        ``out_lse`` ``(bsz, q_head_num)`` float32.  Calls of one engine share its scratch: order them."""
+        self._check(q, (self.bsz, self.q_head_num, self.head_dim), "q", device_only=True)
+        self._check(out, (self.bsz, self.q_head_num, self.head_dim), "out", device_only=True, dense=True)
+        qsb = self._batch_stride(q, self.q_head_num, "q")
+        n_ids = -1
+        if ids is not None:
+            if lens is not None:
+                raise ValueError("lens only limits attention over all rows: give ids or lens")
+            n_ids = self._check_words(ids, (self.bsz, self.kv_head_num, None), "ids")[2]
+        elif self.store_bits != 4:
+            raise ValueError("attention over every stored row needs store_bits=4; give ids")
+        if lens is not None:
+            self._check_words(lens, (self.bsz,), "lens")
+        if out_lse is not None:
+            self._check_words(out_lse, (self.bsz, self.q_head_num), "out_lse")
+        nsb = 0
+        if (k_new is None) != (v_new is None) or (res_k is None) != (res_v is None):
+            raise ValueError("k_new and v_new, res_k and res_v come in pairs")
+        if k_new is not None:
+            for x, what in ((k_new, "k_new"), (v_new, "v_new")):
+                self._check(x, (self.bsz, self.kv_head_num, self.head_dim), what, device_only=True)
+            nsb = self._batch_stride(k_new, self.kv_head_num, "k_new")
+            if self._batch_stride(v_new, self.kv_head_num, "v_new") != nsb:
+                raise ValueError("k_new and v_new must have the same batch stride")
+        sb = sh = 0
+        if int(res_len) < 0:
+            raise ValueError("res_len must not be negative")
+        if res_k is not None:
+            rows = self._check(res_k, (self.bsz, self.kv_head_num, None, self.head_dim), "res_k", device_only=True)[2]
+            self._check(res_v, (self.bsz, self.kv_head_num, rows, self.head_dim), "res_v", device_only=True)
+            need = int(res_len) + (k_new is not None)
+            if rows < need:
+                raise ValueError(f"res_k/res_v hold {rows} rows, the call needs {need}")
+            sb, sh, ss = self._row_strides(res_k, "res_k")
+            if (sb, sh, ss) != self._row_strides(res_v, "res_v") or ss not in (0, self.head_dim):
+                raise ValueError("res_k/res_v must share strides with contiguous rows of head_dim")
+        elif res_len:
+            raise ValueError("res_len > 0 needs res_k and res_v")
+        _lib.check(self._lib.dc_attend_rows(self._h, _ptr(q), qsb, _ptr(ids) if n_ids > 0 else None, n_ids, _ptr(lens),
+                                            _ptr(k_new), _ptr(v_new), nsb, _ptr(res_k), _ptr(res_v), sb, sh, int(res_len),
+                                            float(scale), _ptr(out), _ptr(out_lse), self._stream(stream)))
+
+    def _stream(self, stream) -> int:
+        """The given stream, else the current stream of this engine's device."""
+        if stream is not None:
+            return int(stream)
+        import torch
+
+        return int(torch.cuda.current_stream(self.device).cuda_stream)
+
+    def _check(self, x, shape, what: str, device_only: bool = False, dense: bool = False):
+        """Rows of the element type (or their 16-bit patterns) of this shape (``None``: any); returns the shape."""
+        if _is_torch(x):
+            import torch
+
+            own_type = torch.bfloat16 if self.dtype == BF16 else torch.float16
+            if x.dtype not in (own_type, torch.uint16, torch.int16):
+                raise TypeError(f"{what}: expected {own_type} or 16-bit patterns, got {x.dtype}")
+            if x.is_cuda and x.device.index != self.device:
+                raise ValueError(f"{what} is on {x.device}, the engine on cuda:{self.device}")
+            if device_only and not x.is_cuda:
+                raise ValueError(f"{what} must be a device tensor")
+        else:
+            if device_only:
+                raise TypeError(f"{what} must be a device tensor, got {type(x)}")
+            _require_u16(x, what)
+        got = _shape(x)
+        if len(got) != len(shape) or any(w is not None and g != w for g, w in zip(got, shape)):
+            raise ValueError(f"{what} shape {got} != {tuple('any' if w is None else w for w in shape)}")
+        if dense:
+            _require_contiguous(x, what)
+        return got
+
+    def _check_words(self, x, shape, what: str):
+        """A dense 32-bit device tensor of this shape."""
+        if not _is_torch(x) or not x.is_cuda or x.device.index != self.device:
+            raise ValueError(f"{what} must be a tensor on cuda:{self.device}")
+        import torch
+
+        kinds = (torch.float32,) if what == "out_lse" else (torch.int32, torch.uint32)
+        if x.dtype not in kinds:
+            raise TypeError(f"{what}: expected one of {kinds}, got {x.dtype}")
+        got = _shape(x)
+        if len(got) != len(shape) or any(w is not None and g != w for g, w in zip(got, shape)):
+            raise ValueError(f"{what} shape {got} != {tuple('any' if w is None else w for w in shape)}")
+        _require_contiguous(x, what)
+        return got
+
+    @staticmethod
+    def _row_strides(x, what: str):
+        """Element strides of the (batch, head, row) axes; 0 for an axis of size 1, whose stride is never used."""
+        if isinstance(x, np.ndarray):
+            st = tuple(s // x.itemsize for s in x.strides)
+        else:
+            st = tuple(x.stride())
+        shp = _shape(x)
+        if st[3] != 1 and shp[3] > 1:
+            raise ValueError(f"{what}: head_dim axis must be contiguous")
+        return tuple(0 if n == 1 else int(s) for n, s in zip(shp[:3], st[:3]))
 
     # -- fused device path -----------------------------------------------------------------
     def set_row_offset(self, row_offset: int) -> None:

@@ -16,6 +16,9 @@ so the query never leaves the device:
   still run their own attention kernel;
 * ``decode_attention`` is the fused replacement for query + copy + ``flash_attn_with_kvcache``.
 
+``store_bits=4`` holds the retrieval region in 4 bits (``DiffCacheGPU(store_bits=4)``); the resident
+buffers (sink, window, retrieved rows) stay in the element type.
+
 CUDA graphs.  The reference captures, per layer, one graph ending in ``decode_pre_query_operation``
 and one starting with ``decode_post_query_operation`` (src/diffcache/base.py:116-155) and calls
 ``decode_query_kvcache`` between their replays; both methods here only enqueue copies between
@@ -61,6 +64,7 @@ class DiffCache:
         dtype: str = "bf16",
         device: Optional[int] = None,
         adaptive_budget: bool = False,
+        store_bits: int = 16,
     ) -> None:
         self.num_layers = num_layers
         self.batch_size = batch_size
@@ -111,6 +115,7 @@ class DiffCache:
                 adaptive_budget=adaptive_budget,
                 dtype=dtype,
                 device=self.device.index,
+                store_bits=store_bits,
             )
             for layer_idx in range(num_layers)
         ]

@@ -36,9 +36,10 @@ class AttentionStack:
     def __init__(self, n_layers: int, hidden: int, batch: int, q_heads: int, kv_heads: int, head_dim: int,
                  context: int, topk: int, sink: int, window: int, dtype: str = "bf16", seed: int = 2000,
                  device: Optional[torch.device] = None, group: Optional["dist.ProcessGroup"] = None,
-                 unsharded: bool = False, exchange: str = "nccl"):
+                 unsharded: bool = False, exchange: str = "nccl", store_bits: int = 16):
         """``unsharded=True`` builds the whole stack on this device even inside a process group.
-        ``exchange``: "nccl", "peer" or "auto" (peer when it can be set up)."""
+        ``exchange``: "nccl", "peer" or "auto" (peer when it can be set up).  ``store_bits=4``: the layers' stores
+        hold their rows in 4 bits."""
         use_dist = dist.is_initialized() and not unsharded
         self.world = dist.get_world_size(group) if use_dist else 1
         self.rank = dist.get_rank(group) if use_dist else 0
@@ -72,7 +73,7 @@ class AttentionStack:
             k, v = synth.make_kv(batch, kv_heads, context, head_dim, seed + layer, dtype, device=self.device)
             k, v = k[:, h0:h0 + self.kv_local], v[:, h0:h0 + self.kv_local]
             eng = DiffCacheGPU(batch, self.q_local, self.kv_local, head_dim, max_ctx_len=n_r, dtype=dtype,
-                               device=self.device.index, use_bruteforce=True, name=f"l{layer:03d}")
+                               device=self.device.index, use_bruteforce=True, name=f"l{layer:03d}", store_bits=store_bits)
             eng.prefill(k[:, :, sink:sink + n_r], v[:, :, sink:sink + n_r])
             rk = torch.zeros((batch, self.kv_local, sink + window + 8, head_dim), dtype=dt, device=self.device)
             rv = torch.zeros_like(rk)

@@ -67,6 +67,21 @@ int dc_version(void);
 int dc_create(int bsz, int q_heads, int kv_heads, int head_dim, int64_t max_ctx_len,
               int dtype, int device, dc_engine** out);
 
+/*
+ * An engine whose store holds every row in 4 bits (head_dim / 2 bytes of codes and head_dim / 32 scales of the
+ * element type instead of 2 * head_dim bytes; the format is described with the dc_q4_* functions below).  The
+ * arguments are dc_create's and every engine call works as on a 16-bit store, on the rows as they are read back:
+ * rows are quantised when they are written (dc_prefill, dc_write_rows, dc_insert, the spill of dc_window_push), the
+ * scan ranks s * c, dc_query returns the rows read back, attention runs on the codes.  Only dc_export_rows does not
+ * apply (dc_export_q4).  No counterpart in the reference, whose store is f32 or bf16 in host memory
+ * (diffcache_cpu/src/nsw.rs:47-56).
+ */
+int dc_create_q4(int bsz, int q_heads, int kv_heads, int head_dim, int64_t max_ctx_len,
+                 int dtype, int device, dc_engine** out);
+
+/* 16 or 4; 0 for a NULL engine. */
+int dc_store_bits(dc_engine* e);
+
 /* Frees everything dc_create allocated.  Synchronises the device first. */
 int dc_destroy(dc_engine* e);
 
@@ -101,6 +116,47 @@ int dc_prefill(dc_engine* e, const void* keys, const void* vals, int64_t seq_len
  * appends at the right place on every replay.
  */
 int dc_insert(dc_engine* e, const void* keys, const void* vals, uint64_t stream);
+
+/*
+ * A prefill in pieces: rows [row0, row0 + n) of every problem are written (or overwritten) and ctx_len becomes
+ * max(ctx_len, row0 + n).  keys / vals and strides as in dc_prefill.  row0 may not lie behind the stored rows
+ * (DC_EINVAL), and the call is refused with DC_ESTATE after dc_window_push, when only the device knows where the
+ * stored rows end.  A captured call writes the same positions on every replay.  The reference fills its store in one
+ * piece (lib.rs:329-347).
+ */
+int dc_write_rows(dc_engine* e, const void* keys, const void* vals, int64_t row0, int64_t n, int64_t stride_b,
+                  int64_t stride_h, int64_t stride_s, uint64_t stream);
+
+/*
+ * Reads stored rows back: out[p][i] = row ids[p][i] (ids (bsz*kv_heads, n) on the device), or row row0 + i when ids is
+ * NULL, as (bsz, kv_heads, n, head_dim) of the element type; rows that are not stored (pads 0xFFFFFFFF, ids or
+ * positions >= ctx_len) are zeros.  A 4-bit store gives s * c rounded once.  Device pointers; either output may be
+ * NULL.  The gather of nsw.rs:621-629 for any rows.
+ */
+int dc_read_rows(dc_engine* e, int64_t row0, const uint32_t* ids, int64_t n, void* out_keys, void* out_vals,
+                 uint64_t stream);
+
+/*
+ * Ranking keys bits(65536 - <q, k>) of the stored rows 0 .. min(n, ctx_len) - 1 of every problem into
+ * out_bits[p * out_stride + i] (the rest is left as it was): the scan of nsw.rs:601-607 without the select.  q is
+ * (bsz, kv_heads, head_dim) with q_mode 0 or (bsz, q_heads, head_dim) with q_mode 1 (dc_score_scan).  Device pointers.
+ */
+int dc_score_rows(dc_engine* e, const void* q, int q_mode, int64_t n, uint32_t* out_bits, int64_t out_stride,
+                  uint64_t stream);
+
+/*
+ * Softmax attention of every query head over chosen stored rows, the resident rows and the new token: dc_decode_attend
+ * with the rows given instead of searched.  ids (bsz*kv_heads, n_ids) uint32 row ids (ids that are not stored are
+ * skipped, an id given twice counts twice); n_ids = 0 takes no stored row.  n_ids < 0 (ids NULL): every stored row,
+ * of sequence b only the first lens[b] when lens (bsz int32 on the device) is given; lens beyond ctx_len count as
+ * ctx_len, negative ones as 0; 4-bit stores only (DC_ESTATE otherwise).  Where nothing is left to attend over, out is 0
+ * and out_lse -infinity.  The other arguments are dc_decode_attend_strided's.  Calls of one engine share its scratch:
+ * they must be ordered on the device, captured graphs included.
+ */
+int dc_attend_rows(dc_engine* e, const void* q, int64_t q_stride_b, const uint32_t* ids, int n_ids, const int32_t* lens,
+                   const void* k_new, const void* v_new, int64_t new_stride_b, void* res_k, void* res_v,
+                   int64_t res_stride_b, int64_t res_stride_h, int res_len, float scale, void* out, float* out_lse,
+                   uint64_t stream);
 
 /* Number of valid rows per problem (DataLayer.ctx_len, lib.rs:191).  Synchronises the device after
  * dc_window_push has been used (only the device knows how many rows were spilled into the store). */
@@ -140,6 +196,15 @@ int dc_get_keys(dc_engine* e, float* out);
  * back is dc_prefill (DiffCacheCPU.load, lib.rs:642-644).
  */
 int dc_export_rows(dc_engine* e, void* keys_out, void* vals_out);
+
+/*
+ * Raw copy of a 4-bit store (the snapshot of lib.rs:638-644 for it): codes (bsz, kv_heads, ctx_len, head_dim / 2)
+ * bytes and scales (bsz, kv_heads, ctx_len, head_dim / 32) 16-bit patterns of keys and values, host or device;
+ * synchronous.  dc_import_q4 is the way back and sets ctx_len = n.  DC_ESTATE on a 16-bit engine.
+ */
+int dc_export_q4(dc_engine* e, void* k_codes, void* k_scales, void* v_codes, void* v_scales);
+int dc_import_q4(dc_engine* e, const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,
+                 int64_t n);
 
 /*
  * Replaces DiffCacheCPU.update_r_sq (lib.rs:651-659).  r_sq only enters the
@@ -517,6 +582,52 @@ int dc_adaptive_budget(const uint32_t* sel_bits, int64_t stride, int n_prob, int
 /* Gather rows: out[p][i][:] = store[p][ids[p][i]][:]  (nsw.rs:623-629). */
 int dc_gather_rows(const void* store, int64_t prob_stride, int n_prob, int head_dim,
                    const uint32_t* ids, int64_t ids_stride, int n_ids, void* out, uint64_t stream);
+
+/* ------------------------------------------------------------------------- *
+ * Rows held in 4 bits, stateless (device pointers only): what a dc_create_q4
+ * engine is made of.  No counterpart in the reference.
+ *
+ * Every 32 consecutive elements x of a row form a group with one scale s:
+ *   s = min(round_to_type(max|x| / 7), largest s whose 7-fold is finite),
+ *   s < 2^-126 is stored as 0; a group that holds a NaN or an infinity gets
+ *   s = NaN (and reads back as NaN throughout);
+ *   c = clamp(round_half_even(x / s), -7, 7), 0 where s is 0 or NaN.
+ * A row is read back as s * c; |x - s * c| <= s / 2 (plus the rounding of s at
+ * the group's largest element).  codes: (n_prob, prob_rows, head_dim / 2) bytes,
+ * the nibble c + 8 per element, in an order inside the row that suits the kernels
+ * (csrc/q4.cuh); scales: (n_prob, prob_rows, head_dim / 32) elements.  Both
+ * 16-byte aligned; head_dim 64, 128 or 256.  Channels much larger than the rest
+ * cost precision in their groups; a caller can rotate keys and queries by the
+ * same orthogonal matrix beforehand, which leaves every score as it is.
+ * ------------------------------------------------------------------------- */
+
+/* Rows [row0, row0 + n) of every problem <- keys / vals, strided as in dc_prefill.  Other rows stay as they are. */
+int dc_q4_write_rows(const void* keys, const void* vals, int64_t stride_b, int64_t stride_h, int64_t stride_s, int n_prob,
+                     int kv_heads, int64_t n, int head_dim, int dtype, void* k_codes, void* k_scales, void* v_codes,
+                     void* v_scales, int64_t prob_rows, int64_t row0, uint64_t stream);
+
+/* out[p][i] (n_prob, n, head_dim) = row ids[p * ids_stride + i], or row0 + i when ids is NULL; rows >= n_rows are zeros. */
+int dc_q4_read_rows(const void* codes, const void* scales, int64_t prob_rows, int64_t n_rows, int n_prob, int head_dim,
+                    int dtype, int64_t row0, const uint32_t* ids, int64_t ids_stride, int64_t n, void* out,
+                    uint64_t stream);
+
+/* dc_score_scan over 4-bit keys: dist = 65536 - sum_g s_g sum_{d in g} q_d c_d in fp32 (nsw.rs:129-139 on the rows as
+ * they are read back before rounding). */
+int dc_q4_score_scan(const void* codes, const void* scales, int64_t prob_rows, int n_prob, int64_t n, int head_dim, int dtype,
+                     const void* q, int q_mode, int group, uint32_t* scores, int64_t score_stride, uint32_t* minmax,
+                     uint64_t stream);
+
+/*
+ * dc_sparse_attend over a 4-bit store.  n_sel >= 0: the rows of sel as there.  n_sel < 0 (sel NULL): every row
+ * 0 .. n_rows - 1, of batch b only the first lens[b] when lens (n_prob / kv_heads int32, device) is given.  scratch must
+ * hold dc_q4_attend_scratch_bytes(n_prob, group, head_dim) bytes; calls that overlap on the device need their own.
+ */
+int dc_q4_attend(const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales, int64_t prob_rows,
+                 int64_t n_rows, int n_prob, int kv_heads, int group, int head_dim, int dtype, const void* q,
+                 const uint32_t* sel, int64_t sel_stride, int n_sel, int64_t sel_base, const int32_t* lens, const void* k_new,
+                 const void* v_new, void* res_k, void* res_v, int64_t res_stride_b, int64_t res_stride_h, int res_len,
+                 float scale, void* out, float* out_lse, float* out_acc, float* out_ml, void* scratch, uint64_t stream);
+int64_t dc_q4_attend_scratch_bytes(int n_prob, int group, int head_dim);
 
 /* ------------------------------------------------------------------------- *
  * Product-quantisation baseline (asymmetric distance + exact rerank).
