@@ -17,7 +17,8 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
-constexpr int kHeads = 8;            // query heads of one kv head handled by one CTA
+constexpr int kHeads = 8;            // query heads of one kv head handled by one CTA (columns of the second product)
+constexpr int kTile = 16;            // rows a warp takes at a time
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Args {
@@ -41,147 +42,452 @@ struct Args {
     int res_len;
     const int32_t* res_len_dev;
     float scale_log2;
+    int n_store_split;               // CTAs (per problem and head chunk) that take store rows; the others take 16-bit rows
     int n_split;
     float* part_acc;                 // (n_prob, group, n_split, D)
     float* part_ml;                  // (n_prob, group, n_split, 2)
 };
 
-// grid = (n_split, n_prob, ceil(group / 8)).  A warp takes one row at a time, a lane eight elements of it (one code
-// word), every head's score is a butterfly sum and the softmax runs online per warp; the warps merge at the end.
-template <int DT, int D>
-__global__ void __launch_bounds__(kThreads)
+template <bool BF16>
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if (BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// N 32-bit words from a naturally aligned address, streamed past L1.
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t (&r)[N], const void* p) {
+    if (N == 1) {
+        asm volatile("ld.global.nc.L1::no_allocate.b32 %0, [%1];\n" : "=r"(r[0]) : "l"(p));
+    } else if (N == 2) {
+        asm volatile("ld.global.nc.L1::no_allocate.v2.b32 {%0,%1}, [%2];\n" : "=r"(r[0]), "=r"(r[N > 1 ? 1 : 0]) : "l"(p));
+    } else {
+#pragma unroll
+        for (int i = 0; i + 3 < N; i += 4)
+            asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];\n"
+                         : "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]) : "l"(static_cast<const char*>(p) + 4 * i));
+    }
+}
+
+// Four pairs of codes of a word: pair j = (nibble j, nibble j + 4).  Inserting a nibble into the mantissa of 1024 (fp16) or
+// 128 (bf16) makes it that number plus the nibble, exactly; the offset and the 8 of the encoding go with one operation.
+__device__ __forceinline__ void codes_f16(uint32_t w, uint32_t (&p)[4]) {
+    const uint32_t hi = w >> 8;
+    uint32_t t[4] = {(w & 0x000F000Fu) | 0x64006400u, (w & 0x00F000F0u) | 0x64006400u,
+                     (hi & 0x000F000Fu) | 0x64006400u, (hi & 0x00F000F0u) | 0x64006400u};
+    asm("sub.f16x2 %0, %1, %2;\n" : "=r"(p[0]) : "r"(t[0]), "r"(0x64086408u));                       // - 1032
+    asm("fma.rn.f16x2 %0, %1, %2, %3;\n" : "=r"(p[1]) : "r"(t[1]), "r"(0x2C002C00u), "r"(0xD480D480u));   // / 16 - 72
+    asm("sub.f16x2 %0, %1, %2;\n" : "=r"(p[2]) : "r"(t[2]), "r"(0x64086408u));
+    asm("fma.rn.f16x2 %0, %1, %2, %3;\n" : "=r"(p[3]) : "r"(t[3]), "r"(0x2C002C00u), "r"(0xD480D480u));
+}
+__device__ __forceinline__ void codes_bf16(uint32_t w, uint32_t (&p)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t t = ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
+        asm("sub.bf16x2 %0, %1, %2;\n" : "=r"(p[i]) : "r"(t), "r"(0x43084308u));                      // - 136
+    }
+}
+
+// (x, y) rounded to a pair of 16-bit values, x in the low half; what is lost goes to a second pair.
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+    uint32_t r;
+    if (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(y), "f"(x));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(y), "f"(x));
+    return r;
+}
+template <int DT>
+__device__ __forceinline__ float low_elem(uint32_t w) { return elem_to_float<DT>(static_cast<uint16_t>(w & 0xFFFFu)); }
+template <int DT>
+__device__ __forceinline__ float high_elem(uint32_t w) {
+    return DT == DC_BF16 ? __uint_as_float(w & 0xFFFF0000u) : elem_to_float<DT>(static_cast<uint16_t>(w >> 16));
+}
+
+// Running softmax of the rows one warp has seen.  Lane (g, t) = (lane / 4, lane % 4) works for head g: x[2 * blk + e] is the
+// score of row 4t + 2 blk + e of the tile (log2 units, -inf where there is no row).  On return x holds the weights
+// relative to the new maximum; the return value is the factor the sums so far take.
+__device__ __forceinline__ float softmax_step(float (&x)[4], float& m, float& l) {
+    float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+    mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
+    const float m_new = fmaxf(m, mx);
+    const float alpha = m == -INFINITY ? 0.0f : exp2f(m - m_new);
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = x[i] == -INFINITY ? 0.0f : exp2f(x[i] - m_new);
+    l = l * alpha + (x[0] + x[1]) + (x[2] + x[3]);
+    m = m_new;
+    return alpha;
+}
+
+// o columns are heads 2t, 2t + 1; their factors live in the lanes of rows g = 2t, 2t + 1.
+template <int NT>
+__device__ __forceinline__ void rescale(float (&o)[NT][4], float alpha, int t) {
+    if (!__any_sync(0xFFFFFFFFu, alpha != 1.0f)) return;   // the maximum rarely moves after the first tiles
+    const float a0 = __shfl_sync(0xFFFFFFFFu, alpha, 8 * t), a1 = __shfl_sync(0xFFFFFFFFu, alpha, 8 * t + 4);
+#pragma unroll
+    for (int i = 0; i < NT; i++) { o[i][0] *= a0; o[i][1] *= a1; o[i][2] *= a0; o[i][3] *= a1; }
+}
+
+// One warp's share of a tile of store rows, as loaded: lane (g, t) holds its part of the keys of rows
+// 4 (g / 2) + 2 blk + g % 2 (blk = 0, 1) and of the values and scales of rows 4t .. 4t + 3.
+template <int D>
+struct StoreTile {
+    uint32_t k[2][D / 32], v[4][D / 64], ks[4][D / 64], vs[4][D / 64];
+    uint32_t ok;                     // bit i: row 4t + i exists
+};
+
+// grid = (n_split, n_prob, ceil(group / 8)).
+//
+// Store rows.  S = Q K^T with m16n8k16 MMAs: the query heads are the rows of A, 8 store rows the columns of B.  The codes
+// enter as small integers (fp16, exact), so a group's partial product is exact up to fp32 accumulation and its scale is
+// applied once, in fp32.  The query of a head is normalised by a power of two so that a bf16 query is exact in fp16 too.
+// O^T = V^T P^T: the value codes are A (16 elements of a tile x 16 rows, bf16 integers), the weights are B; a value's scale
+// depends on (row, group) only, so it multiplies the weight, which then enters as a bf16 value and its remainder
+// (16 bits).  With at most four heads value and remainder are two column groups of ONE MMA (columns h and h + 4),
+// otherwise two MMAs.  The rows of a tile are numbered so that a lane's rows in both fragments are 4t .. 4t + 3.
+// All operands go from global memory straight to registers (the stored order of the codes makes every lane's share
+// contiguous), one tile ahead of the arithmetic; warps are independent until the end.
+//
+// 16-bit rows (resident rows, new token): the same two products on the element type, by CTAs of their own.
+template <int DT, int D, bool FEW>
+__global__ void __launch_bounds__(kThreads, D <= 128 ? 3 : 2)
 q4_attend_kernel(const Args a) {
     pdl_launch_dependents();
     pdl_wait();
-    constexpr int WORDS = D / 8;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    constexpr int NT = D / 16;       // 16-element tiles of a row
+    constexpr int NG = D / kQ4Group;
+    constexpr bool BF16 = DT == DC_BF16;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int64_t prob = blockIdx.y;
     const int split = blockIdx.x;
     const int g0 = blockIdx.z * kHeads;
     const int n_heads = min(kHeads, a.group - g0);
     const int b = static_cast<int>(prob / a.kv_heads), h = static_cast<int>(prob % a.kv_heads);
-    const int64_t n_rows = a.n_rows_dev != nullptr ? min(a.n_rows, static_cast<int64_t>(*a.n_rows_dev)) : a.n_rows;
+
+    __shared__ __align__(16) uint16_t s_q[kHeads][D];
+    __shared__ __align__(16) float s_o[kWarps][kHeads][D + 4];
+    __shared__ float s_ml[kWarps][kHeads][2];
+    {
+        const uint16_t* qb = a.q_stride_b ? a.q + b * a.q_stride_b + (static_cast<int64_t>(h) * a.group + g0) * D
+                                          : a.q + (prob * a.group + g0) * D;
+        for (int i = tid; i < kHeads * D / 8; i += kThreads) {
+            const int head = i / (D / 8);
+            reinterpret_cast<uint4*>(&s_q[0][0])[i] =
+                head < n_heads ? reinterpret_cast<const uint4*>(qb)[i] : make_uint4(0, 0, 0, 0);
+        }
+    }
     const int res_len = a.res_len_dev != nullptr ? *a.res_len_dev : a.res_len;
     const int has_new = a.k_new != nullptr ? 1 : 0;
     const int64_t new_off = a.new_stride_b ? b * a.new_stride_b + static_cast<int64_t>(h) * D : prob * D;
-    const bool all_rows = a.n_sel < 0;
-    const uint32_t* sel = a.sel ? a.sel + prob * a.sel_stride : nullptr;
-    const uint16_t* rk = a.res_k ? a.res_k + b * a.res_stride_b + h * a.res_stride_h : nullptr;
-    const uint16_t* rv = a.res_v ? a.res_v + b * a.res_stride_b + h * a.res_stride_h : nullptr;
-    // rows of the store: the first sel_count ids of the list, or rows 0 .. lens[b] - 1
-    int64_t n_store = all_rows ? n_rows : a.n_sel;
-    if (!all_rows && a.sel_count) n_store = max(0, min(a.n_sel, a.sel_count[prob]));
-    if (all_rows && a.lens) n_store = max(static_cast<int64_t>(0), min(n_rows, static_cast<int64_t>(a.lens[b])));
-    const int64_t total = n_store + res_len + has_new;
-    const int64_t per = (total + a.n_split - 1) / a.n_split;
-    const int64_t j0 = min(total, split * per), j1 = min(total, j0 + per);
+    const int64_t res_off = b * a.res_stride_b + h * a.res_stride_h;
+    const uint16_t* qrow = s_q[FEW ? g & 3 : g];   // few heads: rows 4..7 repeat heads 0..3
 
-    if (has_new && split == 0 && blockIdx.z == 0 && rk != nullptr && tid < D / 8) {   // in-place append of the new token
-        const int64_t o = b * a.res_stride_b + h * a.res_stride_h + static_cast<int64_t>(res_len) * D;
-        reinterpret_cast<uint4*>(a.res_k + o)[tid] = reinterpret_cast<const uint4*>(a.k_new + new_off)[tid];
-        reinterpret_cast<uint4*>(a.res_v + o)[tid] = reinterpret_cast<const uint4*>(a.v_new + new_off)[tid];
-    }
-
-    __shared__ float s_q[kHeads][D];
-    __shared__ float s_o[kWarps][kHeads][D];
-    __shared__ float s_ml[kWarps][kHeads][2];
-    const uint16_t* qb = a.q_stride_b ? a.q + b * a.q_stride_b + (static_cast<int64_t>(h) * a.group + g0) * D
-                                      : a.q + (prob * a.group + g0) * D;
-    for (int i = tid; i < kHeads * D; i += kThreads) s_q[i / D][i % D] = i / D < n_heads ? elem_to_float<DT>(qb[i]) : 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    float o[NT][4];
+#pragma unroll
+    for (int i = 0; i < NT; i++) { o[i][0] = 0.0f; o[i][1] = 0.0f; o[i][2] = 0.0f; o[i][3] = 0.0f; }
     __syncthreads();
 
-    // element of the row behind nibble i of this lane's word
-    const int chunk = (lane % WORDS) / (D / 64), w = (lane % WORDS) % (D / 64);
-    auto elem = [&](int i) { const int bt = i >> 1; return 16 * (4 * w + (bt == 1 ? 2 : bt == 2 ? 1 : bt)) + 2 * chunk + (i & 1); };
-    float m[kHeads], l[kHeads], o[kHeads][8];
+    if (split < a.n_store_split) {
+        const bool all_rows = a.n_sel < 0;
+        const int64_t n_rows = a.n_rows_dev != nullptr ? min(a.n_rows, static_cast<int64_t>(*a.n_rows_dev)) : a.n_rows;
+        const uint32_t* sel = a.sel ? a.sel + prob * a.sel_stride : nullptr;
+        // rows of the store: the first sel_count ids of the list, or rows 0 .. lens[b] - 1
+        int64_t n_store = all_rows ? n_rows : a.n_sel;
+        if (!all_rows && a.sel_count) n_store = max(0, min(a.n_sel, a.sel_count[prob]));
+        if (all_rows && a.lens) n_store = max(static_cast<int64_t>(0), min(n_rows, static_cast<int64_t>(a.lens[b])));
+        int64_t per = (n_store + a.n_store_split - 1) / a.n_store_split;
+        per = (per + kTile - 1) / kTile * kTile;
+        const int64_t j0 = min(n_store, split * per), j1 = min(n_store, j0 + per);
+        const uint8_t* kc = a.st.k.codes + prob * a.st.prob_rows * (D / 2) + t * (D / 8);
+        const uint8_t* vc = a.st.v.codes + prob * a.st.prob_rows * (D / 2) + g * (D / 16);
+        const uint16_t* ks = a.st.k.scales + prob * a.st.prob_rows * NG;
+        const uint16_t* vs = a.st.v.scales + prob * a.st.prob_rows * NG;
+
+        // query fragments, normalised to [2^14, 2^15) by a power of two
+        float top = 0.0f;
+        for (int d = t; d < D; d += 4) top = fmaxf(top, fabsf(elem_to_float<DT>(qrow[d])));
+        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+        int ex = static_cast<int>((__float_as_uint(top) >> 23) & 255u);   // 0: zero or subnormal, 255: infinite
+        ex = ex == 255 ? 127 + 14 : max(ex, 28);
+        const float down = __uint_as_float(static_cast<uint32_t>(127 + 14 - ex + 127) << 23);   // 2^(14 - e)
+        const float up = __uint_as_float(static_cast<uint32_t>(ex - 14) << 23) * a.scale_log2;    // 2^(e - 14)
+        uint32_t qa[NT][2];
 #pragma unroll
-    for (int g = 0; g < kHeads; g++) {
-        m[g] = -INFINITY; l[g] = 0.0f;
+        for (int w = 0; w < D / 64; w++)
 #pragma unroll
-        for (int i = 0; i < 8; i++) o[g][i] = 0.0f;
-    }
-    for (int64_t j = j0 + warp; j < j1; j += kWarps) {
-        float kf[8], vf[8];
+            for (int gp = 0; gp < 2; gp++)
 #pragma unroll
-        for (int i = 0; i < 8; i++) { kf[i] = 0.0f; vf[i] = 0.0f; }
-        if (j < n_store) {
-            const int64_t row = all_rows ? j : static_cast<int64_t>(sel[j]) - a.sel_base;
-            if (row < 0 || row >= n_rows) continue;   // pads and ids of other shards
-            const int64_t r = prob * a.st.prob_rows + row;
-            if (lane < WORDS) {
-                const uint32_t kw = reinterpret_cast<const uint32_t*>(a.st.k.codes + r * (D / 2))[lane];
-                const uint32_t vw = reinterpret_cast<const uint32_t*>(a.st.v.codes + r * (D / 2))[lane];
+                for (int c = 0; c < 2; c++) {
+                    const int d = 16 * (4 * w + 2 * gp) + 2 * (2 * t + c);   // a tile's element; + 16 is the group's other tile
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int grp = elem(i) / kQ4Group;
-                    kf[i] = static_cast<float>(static_cast<int>((kw >> (4 * i)) & 15u) - 8) *
-                            elem_to_float<DT>(a.st.k.scales[r * (D / kQ4Group) + grp]);
-                    vf[i] = static_cast<float>(static_cast<int>((vw >> (4 * i)) & 15u) - 8) *
-                            elem_to_float<DT>(a.st.v.scales[r * (D / kQ4Group) + grp]);
+                    for (int e = 0; e < 2; e++)
+                        qa[4 * w + 2 * gp + c][e] = pack2<false>(elem_to_float<DT>(qrow[d + e]) * down,
+                                                                 elem_to_float<DT>(qrow[d + 16 + e]) * down);
+                }
+
+        // this lane's id of a tile's 16 rows (lane and lane + 16 hold the same); -1 where there is no row
+        auto fetch_id = [&](int64_t base) -> int64_t {
+            const int64_t j = base + (lane & 15);
+            if (j >= j1) return -1;
+            if (all_rows) return j;
+            const int64_t row = static_cast<int64_t>(sel[j]) - a.sel_base;
+            return row >= 0 && row < n_rows ? row : -1;   // pads and ids of other shards
+        };
+        auto load = [&](StoreTile<D>& x, int64_t id) {
+#pragma unroll
+            for (int blk = 0; blk < 2; blk++) {
+                const int64_t row = __shfl_sync(0xFFFFFFFFu, id, 4 * (g >> 1) + 2 * blk + (g & 1));
+#pragma unroll
+                for (int i = 0; i < D / 32; i++) x.k[blk][i] = 0;
+                if (row >= 0) load_words<D / 32>(x.k[blk], kc + row * (D / 2));
+            }
+            x.ok = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int64_t row = __shfl_sync(0xFFFFFFFFu, id, 4 * t + i);
+#pragma unroll
+                for (int j = 0; j < D / 64; j++) { x.v[i][j] = 0; x.ks[i][j] = 0; x.vs[i][j] = 0; }
+                if (row >= 0) {
+                    x.ok |= 1u << i;
+                    load_words<D / 64>(x.ks[i], ks + row * NG);
+                    load_words<D / 64>(x.v[i], vc + row * (D / 2));
+                    load_words<D / 64>(x.vs[i], vs + row * NG);
                 }
             }
-        } else {
-            const bool is_res = j < n_store + res_len;
-            const uint16_t* kp = is_res ? rk + (j - n_store) * D : a.k_new + new_off;
-            const uint16_t* vp = is_res ? rv + (j - n_store) * D : a.v_new + new_off;
-            if (lane < WORDS)
+        };
+        auto compute = [&](const StoreTile<D>& x) {
+            float sc[4];
 #pragma unroll
-                for (int i = 0; i < 8; i++) { kf[i] = elem_to_float<DT>(kp[elem(i)]); vf[i] = elem_to_float<DT>(vp[elem(i)]); }
+            for (int blk = 0; blk < 2; blk++) {
+                float acc[NG][4];
+#pragma unroll
+                for (int i = 0; i < NG; i++) { acc[i][0] = 0.0f; acc[i][1] = 0.0f; acc[i][2] = 0.0f; acc[i][3] = 0.0f; }
+#pragma unroll
+                for (int c = 0; c < 2; c++)
+#pragma unroll
+                    for (int w = 0; w < D / 64; w++) {
+                        uint32_t p[4];
+                        codes_f16(x.k[blk][c * (D / 64) + w], p);
+                        mma<false>(acc[2 * w], qa[4 * w + c][0], 0u, qa[4 * w + c][1], 0u, p[0], p[1]);
+                        mma<false>(acc[2 * w + 1], qa[4 * w + 2 + c][0], 0u, qa[4 * w + 2 + c][1], 0u, p[2], p[3]);
+                    }
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    float s = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < D / 64; w++) {
+                        s = fmaf(low_elem<DT>(x.ks[2 * blk + e][w]), acc[2 * w][e], s);
+                        s = fmaf(high_elem<DT>(x.ks[2 * blk + e][w]), acc[2 * w + 1][e], s);
+                    }
+                    sc[2 * blk + e] = (x.ok >> (2 * blk + e)) & 1u ? s * up : -INFINITY;
+                }
+            }
+            rescale<NT>(o, softmax_step(sc, m, l), t);
+#pragma unroll
+            for (int w = 0; w < D / 64; w++) {
+                uint32_t hi[2][2], lo[2][2];   // [group of the word][row block]
+#pragma unroll
+                for (int gp = 0; gp < 2; gp++)
+#pragma unroll
+                    for (int blk = 0; blk < 2; blk++) {
+                        const float p0 = sc[2 * blk] * (gp ? high_elem<DT>(x.vs[2 * blk][w]) : low_elem<DT>(x.vs[2 * blk][w]));
+                        const float p1 = sc[2 * blk + 1] *
+                                         (gp ? high_elem<DT>(x.vs[2 * blk + 1][w]) : low_elem<DT>(x.vs[2 * blk + 1][w]));
+                        const uint32_t r = pack2<true>(p0, p1);
+                        const uint32_t rest = pack2<true>(p0 - low_elem<DC_BF16>(r), p1 - high_elem<DC_BF16>(r));
+                        hi[gp][blk] = FEW && g >= 4 ? rest : r;
+                        lo[gp][blk] = rest;
+                    }
+                // value codes of rows (4t, 4t + 1) and (4t + 2, 4t + 3): nibble pairs of the same element
+                uint32_t va[2][2][4];
+#pragma unroll
+                for (int blk = 0; blk < 2; blk++) {
+                    codes_bf16(__byte_perm(x.v[2 * blk][w], x.v[2 * blk + 1][w], 0x5410), va[blk][0]);   // tiles 4w, 4w + 2
+                    codes_bf16(__byte_perm(x.v[2 * blk][w], x.v[2 * blk + 1][w], 0x7632), va[blk][1]);   // tiles 4w + 1, 4w + 3
+                }
+#pragma unroll
+                for (int tile = 0; tile < 4; tile++) {
+                    const int half = tile & 1, pos = (tile >> 1) * 2, gp = tile >> 1;
+                    mma<true>(o[4 * w + tile], va[0][half][pos], va[0][half][pos + 1], va[1][half][pos], va[1][half][pos + 1],
+                              hi[gp][0], hi[gp][1]);
+                }
+                if (!FEW)
+#pragma unroll
+                    for (int tile = 0; tile < 4; tile++) {
+                        const int half = tile & 1, pos = (tile >> 1) * 2, gp = tile >> 1;
+                        mma<true>(o[4 * w + tile], va[0][half][pos], va[0][half][pos + 1], va[1][half][pos], va[1][half][pos + 1],
+                                  lo[gp][0], lo[gp][1]);
+                    }
+            }
+        };
+        const int64_t step = kWarps * kTile;
+        int64_t base = j0 + warp * kTile;
+        if (base < j1) {
+            StoreTile<D> x;
+            int64_t next_id = fetch_id(base);
+            if (D <= 128) {                            // one tile ahead; at head_dim 256 the registers do not hold two
+                load(x, next_id);
+                next_id = fetch_id(base + step);
+            }
+            for (; base < j1; base += step) {
+                if (D <= 128) {
+                    StoreTile<D> y;
+                    load(y, next_id);                  // nothing is read where the tile lies beyond j1
+                    next_id = fetch_id(base + 2 * step);
+                    compute(x);
+                    x = y;
+                } else {
+                    load(x, next_id);
+                    next_id = fetch_id(base + step);
+                    compute(x);
+                }
+            }
         }
+    } else {
+        // flash-attn's in-place append of the new token (base.py:134-142): one CTA per problem
+        if (has_new && split == a.n_store_split && blockIdx.z == 0 && a.res_k != nullptr && tid < D / 8) {
+            const int64_t off = res_off + static_cast<int64_t>(res_len) * D;
+            reinterpret_cast<uint4*>(a.res_k + off)[tid] = reinterpret_cast<const uint4*>(a.k_new + new_off)[tid];
+            reinterpret_cast<uint4*>(a.res_v + off)[tid] = reinterpret_cast<const uint4*>(a.v_new + new_off)[tid];
+        }
+        const int parts = a.n_split - a.n_store_split, part = split - a.n_store_split;
+        const int total = res_len + has_new;
+        int per = (total + parts - 1) / parts;
+        per = (per + kTile - 1) / kTile * kTile;
+        const int j0 = min(total, part * per), j1 = min(total, j0 + per);
+        uint32_t qa[NT][2];
 #pragma unroll
-        for (int g = 0; g < kHeads; g++) {
-            if (g >= n_heads) continue;
-            float x = 0.0f;
-            if (lane < WORDS)
+        for (int i = 0; i < D / 32; i++) {   // lane t: elements 32 i + 8 t .. + 7 are two k-steps
+            const uint4 w = *reinterpret_cast<const uint4*>(qrow + 32 * i + 8 * t);
+            qa[2 * i][0] = w.x; qa[2 * i][1] = w.y; qa[2 * i + 1][0] = w.z; qa[2 * i + 1][1] = w.w;
+        }
+        auto row_ptr = [&](const uint16_t* res, const uint16_t* fresh, int j) {
+            return j < res_len ? res + res_off + static_cast<int64_t>(j) * D : fresh + new_off;
+        };
+        for (int base = j0 + warp * kTile; base < j1; base += kWarps * kTile) {
+            float sc[4];
 #pragma unroll
-                for (int i = 0; i < 8; i++) x = fmaf(s_q[g][elem(i)], kf[i], x);
+            for (int blk = 0; blk < 2; blk++) {
+                const int j = base + 4 * (g >> 1) + 2 * blk + (g & 1);
+                uint4 kw[D / 32];
 #pragma unroll
-            for (int off = 16; off >= 1; off >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, off);
-            x *= a.scale_log2;
-            const float mn = fmaxf(m[g], x);
-            const float alpha = m[g] == -INFINITY ? 0.0f : exp2f(m[g] - mn);
-            const float p = x == -INFINITY ? 0.0f : exp2f(x - mn);
-            l[g] = l[g] * alpha + p;
-            m[g] = mn;
+                for (int i = 0; i < D / 32; i++) kw[i] = make_uint4(0, 0, 0, 0);
+                if (j < j1) {
+                    const uint16_t* kp = row_ptr(a.res_k, a.k_new, j) + 8 * t;
 #pragma unroll
-            for (int i = 0; i < 8; i++) o[g][i] = o[g][i] * alpha + p * vf[i];
+                    for (int i = 0; i < D / 32; i++) kw[i] = *reinterpret_cast<const uint4*>(kp + 32 * i);
+                }
+                float acc[2][4] = {};
+#pragma unroll
+                for (int i = 0; i < D / 32; i++) {
+                    mma<BF16>(acc[0], qa[2 * i][0], 0u, qa[2 * i][1], 0u, kw[i].x, kw[i].y);
+                    mma<BF16>(acc[1], qa[2 * i + 1][0], 0u, qa[2 * i + 1][1], 0u, kw[i].z, kw[i].w);
+                }
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    sc[2 * blk + e] = base + 4 * t + 2 * blk + e < j1 ? (acc[0][e] + acc[1][e]) * a.scale_log2 : -INFINITY;
+            }
+            uint32_t vw[4][NT];              // rows 4t .. 4t + 3, elements g * D / 8 .. + D / 8
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int j = base + 4 * t + i;
+#pragma unroll
+                for (int n = 0; n < NT; n++) vw[i][n] = 0;
+                if (j < j1) {
+                    const uint16_t* vp = row_ptr(a.res_v, a.v_new, j) + g * (D / 8);
+#pragma unroll
+                    for (int n = 0; n < NT; n += 4) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(vp + 2 * n);
+                        vw[i][n] = w.x; vw[i][n + 1] = w.y; vw[i][n + 2] = w.z; vw[i][n + 3] = w.w;
+                    }
+                }
+            }
+            rescale<NT>(o, softmax_step(sc, m, l), t);
+            uint32_t hi[2], lo[2];
+#pragma unroll
+            for (int blk = 0; blk < 2; blk++) {
+                const uint32_t r = pack2<BF16>(sc[2 * blk], sc[2 * blk + 1]);
+                const uint32_t rest = pack2<BF16>(sc[2 * blk] - low_elem<DT>(r), sc[2 * blk + 1] - high_elem<DT>(r));
+                hi[blk] = FEW && g >= 4 ? rest : r;
+                lo[blk] = rest;
+            }
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                const uint32_t a0 = __byte_perm(vw[0][n], vw[1][n], 0x5410), a1 = __byte_perm(vw[0][n], vw[1][n], 0x7632);
+                const uint32_t a2 = __byte_perm(vw[2][n], vw[3][n], 0x5410), a3 = __byte_perm(vw[2][n], vw[3][n], 0x7632);
+                mma<BF16>(o[n], a0, a1, a2, a3, hi[0], hi[1]);
+                if (!FEW) mma<BF16>(o[n], a0, a1, a2, a3, lo[0], lo[1]);
+            }
         }
     }
+
+    // ---- merge the warps (log-sum-exp) and write this split's partial ----
+    l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
+    l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
+    if (t == 0) { s_ml[warp][g][0] = m; s_ml[warp][g][1] = l; }
 #pragma unroll
-    for (int g = 0; g < kHeads; g++) {
-        if (lane < WORDS)
+    for (int i = 0; i < NT; i++) {
+        if (FEW)   // columns h and h + 4 are the two halves of head h's weights
 #pragma unroll
-            for (int i = 0; i < 8; i++) s_o[warp][g][elem(i)] = o[g][i];
-        if (lane == 0) { s_ml[warp][g][0] = m[g]; s_ml[warp][g][1] = l[g]; }
+            for (int e = 0; e < 4; e++) o[i][e] += __shfl_xor_sync(0xFFFFFFFFu, o[i][e], 2);
+        // this lane's elements (d, d + 1) of the tile, for heads 2t and 2t + 1
+        const int d = split < a.n_store_split ? 16 * i + 2 * g : g * (D / 8) + 2 * i;
+        *reinterpret_cast<float2*>(&s_o[warp][2 * t][d]) = make_float2(o[i][0], o[i][2]);
+        *reinterpret_cast<float2*>(&s_o[warp][2 * t + 1][d]) = make_float2(o[i][1], o[i][3]);
     }
     __syncthreads();
     for (int e = tid; e < n_heads * D; e += kThreads) {
-        const int g = e / D, d = e % D;
+        const int head = e / D, d = e % D;
         float mx = -INFINITY;
-        for (int i = 0; i < kWarps; i++) mx = fmaxf(mx, s_ml[i][g][0]);
+#pragma unroll
+        for (int i = 0; i < kWarps; i++) mx = fmaxf(mx, s_ml[i][head][0]);
         float acc = 0.0f, sum = 0.0f;
+#pragma unroll
         for (int i = 0; i < kWarps; i++) {
-            if (s_ml[i][g][0] == -INFINITY && s_ml[i][g][1] == 0.0f) continue;
-            const float f = exp2f(s_ml[i][g][0] - mx);
-            acc += s_o[i][g][d] * f;
-            sum += s_ml[i][g][1] * f;
+            const float mi = s_ml[i][head][0], li = s_ml[i][head][1];
+            if (mi == -INFINITY && li == 0.0f) continue;   // a warp without rows
+            const float f = exp2f(mi - mx);
+            acc += s_o[i][head][d] * f;
+            sum += li * f;
         }
-        const int64_t slot = (prob * a.group + g0 + g) * a.n_split + split;
+        const int64_t slot = (prob * a.group + g0 + head) * a.n_split + split;
         a.part_acc[slot * D + d] = acc;
         if (d == 0) { a.part_ml[2 * slot] = mx; a.part_ml[2 * slot + 1] = sum; }
     }
 }
 
-int splits(int n_prob, int64_t total_rows) {
-    const int64_t target = std::max(1, 2 * sm_count() / std::max(1, n_prob));
-    const int64_t by_rows = std::max<int64_t>(1, (total_rows + 31) / 32);
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min(target, by_rows), 256)));
+// CTAs per problem (and chunk of 8 heads).  One wave of three CTAs per SM; a 16-bit row counts as three store rows (its
+// 512 bytes at head_dim 128 against 144); every kind of row that occurs gets at least one CTA.
+constexpr int kCtasPerSm = 3;
+constexpr int kMaxSplits = 256;
+
+struct Split { int store, total; };
+
+Split splits(int n_prob, int64_t store_rows, int64_t res_rows) {
+    const int64_t target = std::max(1, kCtasPerSm * sm_count() / std::max(1, n_prob));
+    const int64_t w_store = (store_rows + 63) / 64, w_res = (3 * res_rows + 63) / 64;   // units of 64 store rows
+    const int64_t total = std::max<int64_t>(1, std::min<int64_t>(std::min(target, w_store + w_res), kMaxSplits - 1));
+    int64_t store = 0, res = 0;
+    if (w_store + w_res > 0) {
+        store = w_store > 0 ? std::max<int64_t>(1, (total * w_store + (w_store + w_res) / 2) / (w_store + w_res)) : 0;
+        res = w_res > 0 ? std::max<int64_t>(1, total - store) : 0;
+    }
+    if (store + res == 0) store = 1;
+    return {static_cast<int>(store), static_cast<int>(store + res)};
 }
 
 }  // namespace
 
 int64_t q4_attend_scratch_bytes(int n_prob, int group, int head_dim) {
-    const int64_t ctas = std::min<int64_t>(static_cast<int64_t>(n_prob) * 256, 2ll * sm_count() + n_prob);
+    // splits() makes at most kCtasPerSm * SMs / n_prob + 1 per problem (2 where that is 0 or 1), and at most kMaxSplits
+    const int64_t ctas = std::min<int64_t>(static_cast<int64_t>(n_prob) * kMaxSplits,
+                                           static_cast<int64_t>(kCtasPerSm) * sm_count() + 2ll * n_prob);
     return ctas * group * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
 }
 
@@ -218,21 +524,24 @@ int q4_attend(const Q4Attend& in, cudaStream_t stream) {
     a.res_stride_b = in.res_stride_b; a.res_stride_h = in.res_stride_h;
     a.res_len = in.res_len; a.res_len_dev = in.res_len_dev;
     a.scale_log2 = (in.scale > 0.0f ? in.scale : 1.0f / std::sqrt(static_cast<float>(in.head_dim))) * kLog2e;
-    const int64_t total = (in.n_sel < 0 ? in.n_rows : in.n_sel) + in.res_len + (in.k_new ? 1 : 0);
-    a.n_split = splits(in.n_prob, total);
+    const Split sp = splits(in.n_prob, in.n_sel < 0 ? in.n_rows : in.n_sel, in.res_len + (in.k_new ? 1 : 0));
+    a.n_store_split = sp.store;
+    a.n_split = sp.total;
     a.part_acc = static_cast<float*>(in.scratch);
     a.part_ml = a.part_acc + static_cast<int64_t>(in.n_prob) * a.n_split * in.group * in.head_dim;
     const dim3 grid(static_cast<unsigned>(a.n_split), static_cast<unsigned>(in.n_prob),
                     static_cast<unsigned>((in.group + kHeads - 1) / kHeads));
-#define CASE(DT, D) DC_CUDA_TRY(launch_chained(q4_attend_kernel<DT, D>, grid, dim3(kThreads), 0, stream, 0u, a))
+#define CASE(DT, D)                                                                                                  \
+    if (in.group <= 4) DC_CUDA_TRY(launch_chained(q4_attend_kernel<DT, D, true>, grid, dim3(kThreads), 0, stream, 0u, a)); \
+    else DC_CUDA_TRY(launch_chained(q4_attend_kernel<DT, D, false>, grid, dim3(kThreads), 0, stream, 0u, a))
     if (in.dtype == DC_BF16) {
-        if (in.head_dim == 64) CASE(DC_BF16, 64);
-        else if (in.head_dim == 128) CASE(DC_BF16, 128);
-        else CASE(DC_BF16, 256);
+        if (in.head_dim == 64) { CASE(DC_BF16, 64); }
+        else if (in.head_dim == 128) { CASE(DC_BF16, 128); }
+        else { CASE(DC_BF16, 256); }
     } else {
-        if (in.head_dim == 64) CASE(DC_FP16, 64);
-        else if (in.head_dim == 128) CASE(DC_FP16, 128);
-        else CASE(DC_FP16, 256);
+        if (in.head_dim == 64) { CASE(DC_FP16, 64); }
+        else if (in.head_dim == 128) { CASE(DC_FP16, 128); }
+        else { CASE(DC_FP16, 256); }
     }
 #undef CASE
     return lse_combine(a.part_acc, in.head_dim, static_cast<int64_t>(a.n_split) * in.head_dim, a.part_ml, 2,
