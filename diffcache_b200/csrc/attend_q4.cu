@@ -100,11 +100,33 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
     else asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(y), "f"(x));
     return r;
 }
+// The pair of weights (x, y) as B operand of a head's two column groups: hi = rounded to 16 bits, rest = rounded remainder.
+// With few heads (FEW) the lanes of rows g < 4 need hi, the others rest: `keep_lo` / `keep_hi` are byte selectors that read
+// the rounded halves as floats there, and zeros in the lanes g < 4, so that one expression serves both.
+template <bool BF16, bool FEW>
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t keep_lo, uint32_t keep_hi, uint32_t& hi, uint32_t& rest) {
+    const uint32_t r = pack2<BF16>(x, y);
+    if (BF16) {
+        hi = r;
+        rest = pack2<true>(x - __uint_as_float(__byte_perm(r, 0u, keep_lo)), y - __uint_as_float(__byte_perm(r, 0u, keep_hi)));
+        if (FEW) hi = rest;
+    } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r));
+        rest = pack2<false>(x - f.x, y - f.y);
+        hi = FEW && keep_lo != 0x4444u ? rest : r;
+    }
+}
 template <int DT>
 __device__ __forceinline__ float low_elem(uint32_t w) { return elem_to_float<DT>(static_cast<uint16_t>(w & 0xFFFFu)); }
 template <int DT>
 __device__ __forceinline__ float high_elem(uint32_t w) {
     return DT == DC_BF16 ? __uint_as_float(w & 0xFFFF0000u) : elem_to_float<DT>(static_cast<uint16_t>(w >> 16));
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {   // 2^x to 2 ulp, 0 below 2^-126 and for -inf
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(x));
+    return r;
 }
 
 // Running softmax of the rows one warp has seen.  Lane (g, t) = (lane / 4, lane % 4) works for head g: x[2 * blk + e] is the
@@ -113,13 +135,13 @@ __device__ __forceinline__ float high_elem(uint32_t w) {
 __device__ __forceinline__ float softmax_step(float (&x)[4], float& m, float& l) {
     float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
     mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
-    mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
-    const float m_new = fmaxf(m, mx);
-    const float alpha = m == -INFINITY ? 0.0f : exp2f(m - m_new);
+    mx = fmaxf(fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2)), m);
+    const float ref = mx == -INFINITY ? 0.0f : mx;       // nothing seen yet: every weight is 2^-inf = 0
+    const float alpha = exp2_fast(m - ref);
 #pragma unroll
-    for (int i = 0; i < 4; i++) x[i] = x[i] == -INFINITY ? 0.0f : exp2f(x[i] - m_new);
-    l = l * alpha + (x[0] + x[1]) + (x[2] + x[3]);
-    m = m_new;
+    for (int i = 0; i < 4; i++) x[i] = exp2_fast(x[i] - ref);
+    l = fmaf(l, alpha, (x[0] + x[1]) + (x[2] + x[3]));
+    m = mx;
     return alpha;
 }
 
@@ -137,7 +159,7 @@ __device__ __forceinline__ void rescale(float (&o)[NT][4], float alpha, int t) {
 template <int D>
 struct StoreTile {
     uint32_t k[2][D / 32], v[4][D / 64], ks[4][D / 64], vs[4][D / 64];
-    uint32_t ok;                     // bit i: row 4t + i exists
+    uint32_t ok;                     // bit i: row 4t + i is attended (tiles that may lack rows only)
 };
 
 // grid = (n_split, n_prob, ceil(group / 8)).
@@ -153,7 +175,7 @@ struct StoreTile {
 // contiguous), one tile ahead of the arithmetic; warps are independent until the end.
 //
 // 16-bit rows (resident rows, new token): the same two products on the element type, by CTAs of their own.
-template <int DT, int D, bool FEW>
+template <int DT, int D, bool FEW, bool IDS>
 __global__ void __launch_bounds__(kThreads, D <= 128 ? 3 : 2)
 q4_attend_kernel(const Args a) {
     pdl_launch_dependents();
@@ -186,6 +208,8 @@ q4_attend_kernel(const Args a) {
     const int64_t res_off = b * a.res_stride_b + h * a.res_stride_h;
     const uint16_t* qrow = s_q[FEW ? g & 3 : g];   // few heads: rows 4..7 repeat heads 0..3
 
+    const uint32_t keep_lo = FEW && g < 4 ? 0x4444u : 0x1044u, keep_hi = FEW && g < 4 ? 0x4444u : 0x3244u;
+
     float m = -INFINITY, l = 0.0f;
     float o[NT][4];
 #pragma unroll
@@ -193,13 +217,12 @@ q4_attend_kernel(const Args a) {
     __syncthreads();
 
     if (split < a.n_store_split) {
-        const bool all_rows = a.n_sel < 0;
         const int64_t n_rows = a.n_rows_dev != nullptr ? min(a.n_rows, static_cast<int64_t>(*a.n_rows_dev)) : a.n_rows;
-        const uint32_t* sel = a.sel ? a.sel + prob * a.sel_stride : nullptr;
+        const uint32_t* sel = IDS ? a.sel + prob * a.sel_stride : nullptr;
         // rows of the store: the first sel_count ids of the list, or rows 0 .. lens[b] - 1
-        int64_t n_store = all_rows ? n_rows : a.n_sel;
-        if (!all_rows && a.sel_count) n_store = max(0, min(a.n_sel, a.sel_count[prob]));
-        if (all_rows && a.lens) n_store = max(static_cast<int64_t>(0), min(n_rows, static_cast<int64_t>(a.lens[b])));
+        int64_t n_store = IDS ? (n_rows > 0 ? a.n_sel : 0) : n_rows;
+        if (IDS && a.sel_count) n_store = max(static_cast<int64_t>(0), min(n_store, static_cast<int64_t>(a.sel_count[prob])));
+        if (!IDS && a.lens) n_store = max(static_cast<int64_t>(0), min(n_rows, static_cast<int64_t>(a.lens[b])));
         int64_t per = (n_store + a.n_store_split - 1) / a.n_store_split;
         per = (per + kTile - 1) / kTile * kTile;
         const int64_t j0 = min(n_store, split * per), j1 = min(n_store, j0 + per);
@@ -231,37 +254,47 @@ q4_attend_kernel(const Args a) {
                                                                  elem_to_float<DT>(qrow[d + 16 + e]) * down);
                 }
 
-        // this lane's id of a tile's 16 rows (lane and lane + 16 hold the same); -1 where there is no row
-        auto fetch_id = [&](int64_t base) -> int64_t {
+        // A whole tile of consecutive rows: every address is a lane constant plus the first row.
+        auto load_run = [&](StoreTile<D>& x, int64_t row0) {
+            const uint8_t* kp = kc + (row0 + 4 * (g >> 1) + (g & 1)) * (D / 2);
+            const uint8_t* vp = vc + (row0 + 4 * t) * (D / 2);
+            const uint16_t* ksp = ks + (row0 + 4 * t) * NG;
+            const uint16_t* vsp = vs + (row0 + 4 * t) * NG;
+            load_words<D / 32>(x.k[0], kp);
+            load_words<D / 32>(x.k[1], kp + D);
+#pragma unroll
+            for (int i = 0; i < 4; i++) load_words<D / 64>(x.ks[i], ksp + i * NG);
+#pragma unroll
+            for (int i = 0; i < 4; i++) load_words<D / 64>(x.v[i], vp + i * (D / 2));
+#pragma unroll
+            for (int i = 0; i < 4; i++) load_words<D / 64>(x.vs[i], vsp + i * NG);
+        };
+        // This lane's row of a tile's 16 (lane and lane + 16 hold the same); -1 where there is none.
+        auto fetch_id = [&](int64_t base) -> int32_t {
             const int64_t j = base + (lane & 15);
             if (j >= j1) return -1;
-            if (all_rows) return j;
+            if (!IDS) return static_cast<int32_t>(j);
             const int64_t row = static_cast<int64_t>(sel[j]) - a.sel_base;
-            return row >= 0 && row < n_rows ? row : -1;   // pads and ids of other shards
+            return row >= 0 && row < n_rows ? static_cast<int32_t>(row) : -1;   // pads and ids of other shards
         };
-        auto load = [&](StoreTile<D>& x, int64_t id) {
+        // Any 16 rows; where there is none, row 0 (which exists) is loaded and not used.
+        auto load_any = [&](StoreTile<D>& x, int32_t id) {
+            const int32_t safe = max(id, 0);
+            x.ok = (__ballot_sync(0xFFFFFFFFu, id >= 0) >> (4 * t)) & 15u;
 #pragma unroll
             for (int blk = 0; blk < 2; blk++) {
-                const int64_t row = __shfl_sync(0xFFFFFFFFu, id, 4 * (g >> 1) + 2 * blk + (g & 1));
-#pragma unroll
-                for (int i = 0; i < D / 32; i++) x.k[blk][i] = 0;
-                if (row >= 0) load_words<D / 32>(x.k[blk], kc + row * (D / 2));
+                const int64_t row = __shfl_sync(0xFFFFFFFFu, safe, 4 * (g >> 1) + 2 * blk + (g & 1));
+                load_words<D / 32>(x.k[blk], kc + row * (D / 2));
             }
-            x.ok = 0;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const int64_t row = __shfl_sync(0xFFFFFFFFu, id, 4 * t + i);
-#pragma unroll
-                for (int j = 0; j < D / 64; j++) { x.v[i][j] = 0; x.ks[i][j] = 0; x.vs[i][j] = 0; }
-                if (row >= 0) {
-                    x.ok |= 1u << i;
-                    load_words<D / 64>(x.ks[i], ks + row * NG);
-                    load_words<D / 64>(x.v[i], vc + row * (D / 2));
-                    load_words<D / 64>(x.vs[i], vs + row * NG);
-                }
+                const int64_t row = __shfl_sync(0xFFFFFFFFu, safe, 4 * t + i);
+                load_words<D / 64>(x.ks[i], ks + row * NG);
+                load_words<D / 64>(x.v[i], vc + row * (D / 2));
+                load_words<D / 64>(x.vs[i], vs + row * NG);
             }
         };
-        auto compute = [&](const StoreTile<D>& x) {
+        auto compute = [&](StoreTile<D>& x, bool whole) {
             float sc[4];
 #pragma unroll
             for (int blk = 0; blk < 2; blk++) {
@@ -285,8 +318,17 @@ q4_attend_kernel(const Args a) {
                         s = fmaf(low_elem<DT>(x.ks[2 * blk + e][w]), acc[2 * w][e], s);
                         s = fmaf(high_elem<DT>(x.ks[2 * blk + e][w]), acc[2 * w + 1][e], s);
                     }
-                    sc[2 * blk + e] = (x.ok >> (2 * blk + e)) & 1u ? s * up : -INFINITY;
+                    sc[2 * blk + e] = s * up;
                 }
+            }
+            if (!whole) {   // rows that are not there: no weight, and a scale of 0 in place of whatever was loaded
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (((x.ok >> i) & 1u) == 0) {
+                        sc[i] = -INFINITY;
+#pragma unroll
+                        for (int w = 0; w < D / 64; w++) x.vs[i][w] = 0;
+                    }
             }
             rescale<NT>(o, softmax_step(sc, m, l), t);
 #pragma unroll
@@ -299,10 +341,7 @@ q4_attend_kernel(const Args a) {
                         const float p0 = sc[2 * blk] * (gp ? high_elem<DT>(x.vs[2 * blk][w]) : low_elem<DT>(x.vs[2 * blk][w]));
                         const float p1 = sc[2 * blk + 1] *
                                          (gp ? high_elem<DT>(x.vs[2 * blk + 1][w]) : low_elem<DT>(x.vs[2 * blk + 1][w]));
-                        const uint32_t r = pack2<true>(p0, p1);
-                        const uint32_t rest = pack2<true>(p0 - low_elem<DC_BF16>(r), p1 - high_elem<DC_BF16>(r));
-                        hi[gp][blk] = FEW && g >= 4 ? rest : r;
-                        lo[gp][blk] = rest;
+                        split_pair<true, FEW>(p0, p1, keep_lo, keep_hi, hi[gp][blk], lo[gp][blk]);
                     }
                 // value codes of rows (4t, 4t + 1) and (4t + 2, 4t + 3): nibble pairs of the same element
                 uint32_t va[2][2][4];
@@ -328,25 +367,45 @@ q4_attend_kernel(const Args a) {
         };
         const int64_t step = kWarps * kTile;
         int64_t base = j0 + warp * kTile;
-        if (base < j1) {
-            StoreTile<D> x;
-            int64_t next_id = fetch_id(base);
-            if (D <= 128) {                            // one tile ahead; at head_dim 256 the registers do not hold two
-                load(x, next_id);
-                next_id = fetch_id(base + step);
-            }
-            for (; base < j1; base += step) {
-                if (D <= 128) {
-                    StoreTile<D> y;
-                    load(y, next_id);                  // nothing is read where the tile lies beyond j1
-                    next_id = fetch_id(base + 2 * step);
-                    compute(x);
-                    x = y;
-                } else {
-                    load(x, next_id);
-                    next_id = fetch_id(base + step);
-                    compute(x);
+        if (!IDS) {
+            if (D <= 128 && base + kTile <= j1) {      // one tile ahead, in two sets of registers
+                StoreTile<D> x, y;
+                load_run(x, base);
+                while (true) {
+                    if (base + step + kTile > j1) { compute(x, true); base += step; break; }
+                    load_run(y, base + step);
+                    compute(x, true);
+                    base += step;
+                    if (base + step + kTile > j1) { compute(y, true); base += step; break; }
+                    load_run(x, base + step);
+                    compute(y, true);
+                    base += step;
                 }
+            }
+            StoreTile<D> x;
+            for (; base < j1; base += step) {          // the last tile; every tile where registers do not hold two
+                const bool whole = base + kTile <= j1;
+                if (whole) load_run(x, base);
+                else load_any(x, fetch_id(base));
+                compute(x, whole);
+            }
+        } else if (base < j1) {
+            StoreTile<D> x, y;
+            load_any(x, fetch_id(base));
+            int32_t id = fetch_id(base + step);
+            while (true) {
+                bool more = base + step < j1;
+                if (D <= 128 && more) { load_any(y, id); id = fetch_id(base + 2 * step); }
+                compute(x, __all_sync(0xFFFFFFFFu, x.ok == 15u));
+                if (!more) break;
+                base += step;
+                more = base + step < j1;
+                if (D > 128) { load_any(y, id); id = fetch_id(base + step); }
+                else if (more) { load_any(x, id); id = fetch_id(base + 2 * step); }
+                compute(y, __all_sync(0xFFFFFFFFu, y.ok == 15u));
+                if (!more) break;
+                base += step;
+                if (D > 128) { load_any(x, id); id = fetch_id(base + step); }
             }
         }
     } else {
@@ -412,10 +471,7 @@ q4_attend_kernel(const Args a) {
             uint32_t hi[2], lo[2];
 #pragma unroll
             for (int blk = 0; blk < 2; blk++) {
-                const uint32_t r = pack2<BF16>(sc[2 * blk], sc[2 * blk + 1]);
-                const uint32_t rest = pack2<BF16>(sc[2 * blk] - low_elem<DT>(r), sc[2 * blk + 1] - high_elem<DT>(r));
-                hi[blk] = FEW && g >= 4 ? rest : r;
-                lo[blk] = rest;
+                split_pair<BF16, FEW>(sc[2 * blk], sc[2 * blk + 1], keep_lo, keep_hi, hi[blk], lo[blk]);
             }
 #pragma unroll
             for (int n = 0; n < NT; n++) {
@@ -531,9 +587,10 @@ int q4_attend(const Q4Attend& in, cudaStream_t stream) {
     a.part_ml = a.part_acc + static_cast<int64_t>(in.n_prob) * a.n_split * in.group * in.head_dim;
     const dim3 grid(static_cast<unsigned>(a.n_split), static_cast<unsigned>(in.n_prob),
                     static_cast<unsigned>((in.group + kHeads - 1) / kHeads));
-#define CASE(DT, D)                                                                                                  \
-    if (in.group <= 4) DC_CUDA_TRY(launch_chained(q4_attend_kernel<DT, D, true>, grid, dim3(kThreads), 0, stream, 0u, a)); \
-    else DC_CUDA_TRY(launch_chained(q4_attend_kernel<DT, D, false>, grid, dim3(kThreads), 0, stream, 0u, a))
+#define LAUNCH(DT, D, FEW, IDS) DC_CUDA_TRY(launch_chained(q4_attend_kernel<DT, D, FEW, IDS>, grid, dim3(kThreads), 0, stream, 0u, a))
+#define CASE(DT, D)                                                                                   \
+    if (in.group <= 4) { if (in.n_sel < 0) LAUNCH(DT, D, true, false); else LAUNCH(DT, D, true, true); } \
+    else { if (in.n_sel < 0) LAUNCH(DT, D, false, false); else LAUNCH(DT, D, false, true); }
     if (in.dtype == DC_BF16) {
         if (in.head_dim == 64) { CASE(DC_BF16, 64); }
         else if (in.head_dim == 128) { CASE(DC_BF16, 128); }
@@ -544,6 +601,7 @@ int q4_attend(const Q4Attend& in, cudaStream_t stream) {
         else { CASE(DC_FP16, 256); }
     }
 #undef CASE
+#undef LAUNCH
     return lse_combine(a.part_acc, in.head_dim, static_cast<int64_t>(a.n_split) * in.head_dim, a.part_ml, 2,
                        static_cast<int64_t>(a.n_split) * 2, a.n_split, static_cast<int64_t>(in.n_prob) * in.group, in.head_dim,
                        in.dtype, in.out, in.out_lse, in.out_acc, in.out_ml, stream, nullptr, in.xout, in.fin, true);

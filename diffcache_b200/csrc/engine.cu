@@ -913,7 +913,6 @@ int dc_read_rows(dc_engine* e, int64_t row0, const uint32_t* ids, int64_t n, voi
                static_cast<long long>(row0), static_cast<long long>(row0), static_cast<long long>(n),
                static_cast<long long>(e->max_ctx));
     if (n == 0 || (out_keys == nullptr && out_vals == nullptr)) return DC_OK;
-    DC_REQUIRE(is_device_ptr(ids) && is_device_ptr(out_keys) && is_device_ptr(out_vals), "dc_read_rows: device pointers only");
     DC_REQUIRE(((reinterpret_cast<uintptr_t>(out_keys) | reinterpret_cast<uintptr_t>(out_vals)) & 15) == 0 &&
                    (reinterpret_cast<uintptr_t>(ids) & 3) == 0,
                "dc_read_rows: outputs must be 16-byte aligned");
@@ -937,7 +936,6 @@ int dc_score_rows(dc_engine* e, const void* q, int q_mode, int64_t n, uint32_t* 
                static_cast<long long>(n), static_cast<long long>(out_stride), static_cast<long long>(e->max_ctx));
     DC_REQUIRE((reinterpret_cast<uintptr_t>(q) & 15) == 0 && (reinterpret_cast<uintptr_t>(out_bits) & 3) == 0,
                "dc_score_rows: q must be 16-byte aligned");
-    DC_REQUIRE(is_device_ptr(q) && is_device_ptr(out_bits), "dc_score_rows: device pointers only");
     cudaStream_t s = as_stream(stream);
     if (e->q4)   // the kernel clamps n to the rows stored when it runs
         return q4_score_scan(e->st.k, e->st.prob_rows, e->n_prob, n, e->head_dim, e->dtype, q, q_mode, e->group, out_bits,
@@ -963,9 +961,6 @@ int dc_attend_rows(dc_engine* e, const void* q, int64_t q_stride_b, const uint32
                "dc_attend_rows: q batch stride smaller than one batch of query heads");
     DC_REQUIRE(new_stride_b == 0 || new_stride_b >= static_cast<int64_t>(e->kv_heads) * e->head_dim,
                "dc_attend_rows: k_new/v_new batch stride smaller than one batch of kv heads");
-    DC_REQUIRE(is_device_ptr(q) && is_device_ptr(ids) && is_device_ptr(lens) && is_device_ptr(out) && is_device_ptr(k_new) &&
-                   is_device_ptr(v_new) && is_device_ptr(res_k) && is_device_ptr(res_v) && is_device_ptr(out_lse),
-               "dc_attend_rows: device pointers only");
     if (n_ids < 0 && !e->q4) {
         set_error("dc_attend_rows: attention over every stored row needs a 4-bit store (dc_create_q4)");
         return DC_ESTATE;

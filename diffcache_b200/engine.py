@@ -9,6 +9,7 @@ a numpy array (host) or a torch tensor (host or CUDA).
 from __future__ import annotations
 
 import ctypes
+import functools
 import time
 from typing import Optional, Sequence
 
@@ -90,6 +91,44 @@ def _current_stream(stream) -> int:
     import torch
 
     return int(torch.cuda.current_stream().cuda_stream)
+
+
+@functools.lru_cache(maxsize=None)
+def _element_types():
+    import torch
+
+    return {BF16: (torch.bfloat16, torch.uint16, torch.int16), FP16: (torch.float16, torch.uint16, torch.int16)}
+
+
+@functools.lru_cache(maxsize=None)
+def _word_types(floats: bool):
+    import torch
+
+    return (torch.float32,) if floats else (torch.int32, torch.uint32)
+
+
+@functools.lru_cache(maxsize=None)
+def _raw_stream_getter():
+    import torch
+
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # a tenth of the time of building a Stream object
+    return raw if raw is not None else lambda device: torch.cuda.current_stream(device).cuda_stream
+
+
+def _device_stream(device: int) -> int:
+    return int(_raw_stream_getter()(device))
+
+
+def _row_strides(x, what: str):
+    """Element strides of the (batch, head, row) axes; 0 for an axis of size 1, whose stride is never used."""
+    if isinstance(x, np.ndarray):
+        st = tuple(s // x.itemsize for s in x.strides)
+    else:
+        st = x.stride()
+    shp = x.shape
+    if st[3] != 1 and shp[3] > 1:
+        raise ValueError(f"{what}: head_dim axis must be contiguous")
+    return (st[0] if shp[0] != 1 else 0, st[1] if shp[1] != 1 else 0, st[2] if shp[2] != 1 else 0)
 
 
 class DiffCacheGPU:
@@ -274,13 +313,12 @@ class DiffCacheGPU:
         """Writes (or overwrites) stored rows ``[row0, row0 + n)``, e.g. one chunk of a chunked prefill;
         ``keys``/``vals`` ``(bsz, kv_head_num, n, head_dim)`` as in :meth:`prefill`.  ``row0`` may be at most
         ``ctx_len``; the store then holds ``max(ctx_len, row0 + n)`` rows."""
-        shape = (self.bsz, self.kv_head_num, None, self.head_dim)
-        n = self._check(keys, shape, "keys")[2]
-        self._check(vals, (self.bsz, self.kv_head_num, n, self.head_dim), "vals")
-        sk, sv = self._row_strides(keys, "keys"), self._row_strides(vals, "vals")
-        if sk != sv:
+        n = self._rows(keys, None, "keys")
+        self._rows(vals, n, "vals")
+        sb, sh, ss = _row_strides(keys, "keys")
+        if _row_strides(vals, "vals") != (sb, sh, ss):
             raise ValueError("keys and vals must share one stride pattern")
-        _lib.check(self._lib.dc_write_rows(self._h, _ptr(keys), _ptr(vals), int(row0), n, *sk, self._stream(stream)))
+        _lib.check(self._lib.dc_write_rows(self._h, _ptr(keys), _ptr(vals), int(row0), n, sb, sh, ss, self._stream(stream)))
 
     def read_rows(self, out_keys, out_vals, row0: int = 0, ids=None, stream=None) -> None:
         """Reads stored rows back into ``out_keys``/``out_vals`` ``(bsz, kv_head_num, n, head_dim)`` (dense device
@@ -289,11 +327,13 @@ class DiffCacheGPU:
         n = None
         for x, what in ((out_keys, "out_keys"), (out_vals, "out_vals")):
             if x is not None:
-                n = self._check(x, (self.bsz, self.kv_head_num, n, self.head_dim), what, device_only=True, dense=True)[2]
+                self._on_device(x, what)
+                n = self._rows(x, n, what)
+                _require_contiguous(x, what)
         if n is None:
             return
         if ids is not None:
-            self._check_words(ids, (self.bsz, self.kv_head_num, n), "ids")
+            self._words(ids, (self.bsz, self.kv_head_num, n), "ids")
         _lib.check(self._lib.dc_read_rows(self._h, int(row0), _ptr(ids), n, _ptr(out_keys), _ptr(out_vals),
                                           self._stream(stream)))
 
@@ -302,12 +342,11 @@ class DiffCacheGPU:
         n)`` (32-bit device tensor; entries beyond the stored rows stay as they are).  ``q`` ``(bsz, kv_head_num,
         head_dim)`` holds one (group-mean) vector per kv head, or ``(bsz, q_head_num, head_dim)`` the query
         heads, whose group mean is taken."""
-        heads = _shape(q)[1] if len(_shape(q)) == 3 else -1
-        mode = 0 if heads == self.kv_head_num else 1
-        self._check(q, (self.bsz, self.kv_head_num if mode == 0 else self.q_head_num, self.head_dim), "q", device_only=True,
-                    dense=True)
-        n = self._check_words(out_bits, (self.bsz, self.kv_head_num, None), "out_bits")[2]
-        _lib.check(self._lib.dc_score_rows(self._h, _ptr(q), mode, n, _ptr(out_bits), n, self._stream(stream)))
+        mode = 0 if len(q.shape) == 3 and q.shape[1] == self.kv_head_num else 1
+        self._heads(q, self.kv_head_num if mode == 0 else self.q_head_num, "q")
+        _require_contiguous(q, "q")
+        n = self._words(out_bits, (self.bsz, self.kv_head_num, None), "out_bits")
+        _lib.check(self._lib.dc_score_rows(self._h, q.data_ptr(), mode, n, out_bits.data_ptr(), n, self._stream(stream)))
 
     def attend_rows(self, q, out, ids=None, lens=None, res_k=None, res_v=None, res_len: int = 0, k_new=None, v_new=None,
                     scale: float = 0.0, out_lse=None, stream=None) -> None:
@@ -316,104 +355,100 @@ class DiffCacheGPU:
         Without ``ids`` (4-bit stores): every stored row, of sequence ``b`` only the first ``lens[b]`` (int32
         device tensor ``(bsz,)``) when ``lens`` is given.  Heads that have nothing to attend over get 0, and -inf in
         ``out_lse`` ``(bsz, q_head_num)`` float32.  Calls of one engine share its scratch: order them."""
-        self._check(q, (self.bsz, self.q_head_num, self.head_dim), "q", device_only=True)
-        self._check(out, (self.bsz, self.q_head_num, self.head_dim), "out", device_only=True, dense=True)
-        qsb = self._batch_stride(q, self.q_head_num, "q")
-        n_ids = -1
+        self._heads(q, self.q_head_num, "q")
+        self._heads(out, self.q_head_num, "out")
+        _require_contiguous(out, "out")
+        qsb = 0 if q.is_contiguous() else self._batch_stride(q, self.q_head_num, "q")
+        n_ids, ids_ptr, lens_ptr, lse_ptr, kn_ptr, vn_ptr, nsb, rk_ptr, rv_ptr, sb, sh = -1, None, None, None, None, None, 0, None, None, 0, 0
         if ids is not None:
             if lens is not None:
                 raise ValueError("lens only limits attention over all rows: give ids or lens")
-            n_ids = self._check_words(ids, (self.bsz, self.kv_head_num, None), "ids")[2]
+            n_ids = self._words(ids, (self.bsz, self.kv_head_num, None), "ids")
+            ids_ptr = ids.data_ptr() if n_ids > 0 else None
         elif self.store_bits != 4:
             raise ValueError("attention over every stored row needs store_bits=4; give ids")
-        if lens is not None:
-            self._check_words(lens, (self.bsz,), "lens")
+        elif lens is not None:
+            self._words(lens, (self.bsz,), "lens")
+            lens_ptr = lens.data_ptr()
         if out_lse is not None:
-            self._check_words(out_lse, (self.bsz, self.q_head_num), "out_lse")
-        nsb = 0
+            self._words(out_lse, (self.bsz, self.q_head_num), "out_lse")
+            lse_ptr = out_lse.data_ptr()
         if (k_new is None) != (v_new is None) or (res_k is None) != (res_v is None):
             raise ValueError("k_new and v_new, res_k and res_v come in pairs")
-        if k_new is not None:
-            for x, what in ((k_new, "k_new"), (v_new, "v_new")):
-                self._check(x, (self.bsz, self.kv_head_num, self.head_dim), what, device_only=True)
-            nsb = self._batch_stride(k_new, self.kv_head_num, "k_new")
-            if self._batch_stride(v_new, self.kv_head_num, "v_new") != nsb:
-                raise ValueError("k_new and v_new must have the same batch stride")
-        sb = sh = 0
-        if int(res_len) < 0:
+        need = int(res_len)
+        if need < 0:
             raise ValueError("res_len must not be negative")
+        if k_new is not None:
+            self._heads(k_new, self.kv_head_num, "k_new")
+            self._heads(v_new, self.kv_head_num, "v_new")
+            if not (k_new.is_contiguous() and v_new.is_contiguous()):
+                nsb = self._batch_stride(k_new, self.kv_head_num, "k_new")
+                if self._batch_stride(v_new, self.kv_head_num, "v_new") != nsb:
+                    raise ValueError("k_new and v_new must have the same batch stride")
+            kn_ptr, vn_ptr = k_new.data_ptr(), v_new.data_ptr()
+            need += 1
         if res_k is not None:
-            rows = self._check(res_k, (self.bsz, self.kv_head_num, None, self.head_dim), "res_k", device_only=True)[2]
-            self._check(res_v, (self.bsz, self.kv_head_num, rows, self.head_dim), "res_v", device_only=True)
-            need = int(res_len) + (k_new is not None)
+            self._on_device(res_k, "res_k")
+            self._on_device(res_v, "res_v")
+            rows = self._rows(res_k, None, "res_k")
+            self._rows(res_v, rows, "res_v")
             if rows < need:
                 raise ValueError(f"res_k/res_v hold {rows} rows, the call needs {need}")
-            sb, sh, ss = self._row_strides(res_k, "res_k")
-            if (sb, sh, ss) != self._row_strides(res_v, "res_v") or ss not in (0, self.head_dim):
+            sb, sh, ss = _row_strides(res_k, "res_k")
+            if (sb, sh, ss) != _row_strides(res_v, "res_v") or ss not in (0, self.head_dim):
                 raise ValueError("res_k/res_v must share strides with contiguous rows of head_dim")
+            rk_ptr, rv_ptr = res_k.data_ptr(), res_v.data_ptr()
         elif res_len:
             raise ValueError("res_len > 0 needs res_k and res_v")
-        _lib.check(self._lib.dc_attend_rows(self._h, _ptr(q), qsb, _ptr(ids) if n_ids > 0 else None, n_ids, _ptr(lens),
-                                            _ptr(k_new), _ptr(v_new), nsb, _ptr(res_k), _ptr(res_v), sb, sh, int(res_len),
-                                            float(scale), _ptr(out), _ptr(out_lse), self._stream(stream)))
+        _lib.check(self._lib.dc_attend_rows(self._h, q.data_ptr(), qsb, ids_ptr, n_ids, lens_ptr, kn_ptr, vn_ptr, nsb, rk_ptr, rv_ptr,
+                                            sb, sh, int(res_len), scale, out.data_ptr(), lse_ptr, self._stream(stream)))
 
+    # Argument checks of the calls above.  They are the larger part of a small call's time, so each looks at an
+    # attribute once.
     def _stream(self, stream) -> int:
         """The given stream, else the current stream of this engine's device."""
-        if stream is not None:
-            return int(stream)
-        import torch
+        return _device_stream(self.device) if stream is None else int(stream)
 
-        return int(torch.cuda.current_stream(self.device).cuda_stream)
+    def _on_device(self, x, what: str) -> None:
+        if not _is_torch(x):
+            raise TypeError(f"{what} must be a device tensor, got {type(x)}")
+        if x.get_device() != self.device:   # -1 for host tensors
+            raise ValueError(f"{what} must be a device tensor on cuda:{self.device}, got one on {x.device}")
 
-    def _check(self, x, shape, what: str, device_only: bool = False, dense: bool = False):
-        """Rows of the element type (or their 16-bit patterns) of this shape (``None``: any); returns the shape."""
+    def _rows(self, x, n, what: str) -> int:
+        """Rows (bsz, kv_head_num, n, head_dim) of the element type or its 16-bit patterns, in host memory or on this
+        engine's device; n None: any.  Returns n."""
         if _is_torch(x):
-            import torch
-
-            own_type = torch.bfloat16 if self.dtype == BF16 else torch.float16
-            if x.dtype not in (own_type, torch.uint16, torch.int16):
-                raise TypeError(f"{what}: expected {own_type} or 16-bit patterns, got {x.dtype}")
-            if x.is_cuda and x.device.index != self.device:
+            if x.dtype not in _element_types()[self.dtype]:
+                raise TypeError(f"{what}: expected {_element_types()[self.dtype][0]} or 16-bit patterns, got {x.dtype}")
+            if x.get_device() not in (-1, self.device):
                 raise ValueError(f"{what} is on {x.device}, the engine on cuda:{self.device}")
-            if device_only and not x.is_cuda:
-                raise ValueError(f"{what} must be a device tensor")
         else:
-            if device_only:
-                raise TypeError(f"{what} must be a device tensor, got {type(x)}")
             _require_u16(x, what)
-        got = _shape(x)
-        if len(got) != len(shape) or any(w is not None and g != w for g, w in zip(got, shape)):
+        shape = x.shape
+        if len(shape) != 4 or shape[0] != self.bsz or shape[1] != self.kv_head_num or shape[3] != self.head_dim or n not in (None, shape[2]):
+            raise ValueError(f"{what} shape {tuple(shape)} != {(self.bsz, self.kv_head_num, 'any' if n is None else n, self.head_dim)}")
+        return shape[2]
+
+    def _heads(self, x, heads: int, what: str) -> None:
+        """(bsz, heads, head_dim) of the element type on this engine's device."""
+        self._on_device(x, what)
+        if x.dtype not in _element_types()[self.dtype]:
+            raise TypeError(f"{what}: expected {_element_types()[self.dtype][0]} or 16-bit patterns, got {x.dtype}")
+        if x.shape != (self.bsz, heads, self.head_dim):
+            raise ValueError(f"{what} shape {tuple(x.shape)} != {(self.bsz, heads, self.head_dim)}")
+
+    def _words(self, x, shape, what: str) -> int:
+        """A dense 32-bit tensor of this shape (last size None: any) on this engine's device; returns its last size."""
+        self._on_device(x, what)
+        if x.dtype not in _word_types(what == "out_lse"):
+            raise TypeError(f"{what}: expected one of {_word_types(what == 'out_lse')}, got {x.dtype}")
+        got = tuple(x.shape)
+        if got != shape and (shape[-1] is not None or len(got) != len(shape) or got[:-1] != shape[:-1]):
             raise ValueError(f"{what} shape {got} != {tuple('any' if w is None else w for w in shape)}")
-        if dense:
-            _require_contiguous(x, what)
-        return got
-
-    def _check_words(self, x, shape, what: str):
-        """A dense 32-bit device tensor of this shape."""
-        if not _is_torch(x) or not x.is_cuda or x.device.index != self.device:
-            raise ValueError(f"{what} must be a tensor on cuda:{self.device}")
-        import torch
-
-        kinds = (torch.float32,) if what == "out_lse" else (torch.int32, torch.uint32)
-        if x.dtype not in kinds:
-            raise TypeError(f"{what}: expected one of {kinds}, got {x.dtype}")
-        got = _shape(x)
-        if len(got) != len(shape) or any(w is not None and g != w for g, w in zip(got, shape)):
-            raise ValueError(f"{what} shape {got} != {tuple('any' if w is None else w for w in shape)}")
-        _require_contiguous(x, what)
-        return got
-
-    @staticmethod
-    def _row_strides(x, what: str):
-        """Element strides of the (batch, head, row) axes; 0 for an axis of size 1, whose stride is never used."""
-        if isinstance(x, np.ndarray):
-            st = tuple(s // x.itemsize for s in x.strides)
-        else:
-            st = tuple(x.stride())
-        shp = _shape(x)
-        if st[3] != 1 and shp[3] > 1:
-            raise ValueError(f"{what}: head_dim axis must be contiguous")
-        return tuple(0 if n == 1 else int(s) for n, s in zip(shp[:3], st[:3]))
+        if not x.is_contiguous():
+            raise ValueError(f"{what} must be C-contiguous")
+        return got[-1]
 
     # -- fused device path -----------------------------------------------------------------
     def set_row_offset(self, row_offset: int) -> None:
