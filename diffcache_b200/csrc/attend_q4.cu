@@ -20,6 +20,13 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kHeads = 8;            // query heads of one kv head handled by one CTA (columns of the second product)
 constexpr int kTile = 16;            // rows a warp takes at a time
 constexpr float kLog2e = 1.4426950408889634f;
+#ifndef Q4_C
+#define Q4_C 3
+#endif
+#ifndef Q4_S
+#define Q4_S 4
+#endif
+__host__ __device__ constexpr int ctas_per_sm(int head_dim) { return head_dim <= 128 ? Q4_C : 2; }
 
 struct Args {
     Q4Store st;
@@ -58,19 +65,66 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// N 32-bit words from a naturally aligned address, streamed past L1.
+// The first product of a sum: nothing to add to.
+template <bool BF16>
+__device__ __forceinline__ void mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if (BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+// ---- a tile of 16 store rows in shared memory, private to one warp ----
+// Asynchronous copies of 16 (codes) and 4 / 8 / 16 bytes (a row's scales); with `ok` false zeros are written instead.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(unsigned dst, const void* src) {
+    if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;\n" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
+template <int BYTES>
+__device__ __forceinline__ void copy_async(unsigned dst, const void* src, bool ok) {
+    const int n = ok ? BYTES : 0;
+    if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(n) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;\n" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
 template <int N>
-__device__ __forceinline__ void load_words(uint32_t (&r)[N], const void* p) {
-    if (N == 1) {
-        asm volatile("ld.global.nc.L1::no_allocate.b32 %0, [%1];\n" : "=r"(r[0]) : "l"(p));
-    } else if (N == 2) {
-        asm volatile("ld.global.nc.L1::no_allocate.v2.b32 {%0,%1}, [%2];\n" : "=r"(r[0]), "=r"(r[N > 1 ? 1 : 0]) : "l"(p));
-    } else {
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
+
+template <int N>
+__device__ __forceinline__ void lds_words(uint32_t (&r)[N], unsigned addr) {
+    if (N == 1) asm volatile("ld.shared.b32 %0, [%1];\n" : "=r"(r[0]) : "r"(addr));
+    else if (N == 2) asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];\n" : "=r"(r[0]), "=r"(r[N > 1 ? 1 : 0]) : "r"(addr));
+    else
 #pragma unroll
         for (int i = 0; i + 3 < N; i += 4)
-            asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];\n"
-                         : "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]) : "l"(static_cast<const char*>(p) + 4 * i));
+            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];\n"
+                         : "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]) : "r"(addr + 4 * i));
+}
+
+template <int D>
+struct Ring {
+    static constexpr int CODES = kTile * (D / 2);        // one tensor's codes of a tile
+    static constexpr int SCALES = kTile * (D / 16);
+    static constexpr int STAGE = 2 * CODES + 2 * SCALES; // [K codes | V codes | K scales | V scales]
+    static constexpr int STAGES = Q4_S;
+    // Byte of 16-byte chunk c of row r among a tile's codes.  Rows and chunks are permuted so that neither the keys (eight
+    // rows, a quarter row per lane) nor the values (rows 4t + i, an eighth per lane) make a warp's lanes share banks.
+    __device__ static __forceinline__ int chunk(int r, int c) {
+        if (D == 64) return ((r & ~3) | ((r & 3) ^ (r >> 2))) * 32 + c * 16;
+        if (D == 128) return (r ^ ((r >> 2) & 1)) * 64 + ((c ^ (r >> 2)) & 3) * 16;
+        return r * 128 + ((c ^ (2 * (r >> 2)) ^ (r & 1)) & 7) * 16;
     }
+};
+template <int D>
+constexpr size_t attend_smem_bytes() {
+    const size_t ring = static_cast<size_t>(kWarps) * Ring<D>::STAGES * Ring<D>::STAGE;
+    const size_t merge = static_cast<size_t>(kWarps) * kHeads * (D + 4) * sizeof(float);
+    return ring > merge ? ring : merge;
 }
 
 // Four pairs of codes of a word: pair j = (nibble j, nibble j + 4).  Inserting a nibble into the mantissa of 1024 (fp16) or
@@ -129,38 +183,49 @@ __device__ __forceinline__ float exp2_fast(float x) {   // 2^x to 2 ulp, 0 below
     return r;
 }
 
-// Running softmax of the rows one warp has seen.  Lane (g, t) = (lane / 4, lane % 4) works for head g: x[2 * blk + e] is the
-// score of row 4t + 2 blk + e of the tile (log2 units, -inf where there is no row).  On return x holds the weights
-// relative to the new maximum; the return value is the factor the sums so far take.
-__device__ __forceinline__ float softmax_step(float (&x)[4], float& m, float& l) {
-    float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-    mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
-    mx = fmaxf(fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2)), m);
-    const float ref = mx == -INFINITY ? 0.0f : mx;       // nothing seen yet: every weight is 2^-inf = 0
-    const float alpha = exp2_fast(m - ref);
-#pragma unroll
-    for (int i = 0; i < 4; i++) x[i] = exp2_fast(x[i] - ref);
-    l = fmaf(l, alpha, (x[0] + x[1]) + (x[2] + x[3]));
-    m = mx;
-    return alpha;
-}
-
-// o columns are heads 2t, 2t + 1; their factors live in the lanes of rows g = 2t, 2t + 1.
+// Running softmax of the rows one warp has seen.  Lane (g, t) = (lane / 4, lane % 4) holds the scores x[2 * blk + e] of two
+// rows (blk) of the tile for heads 2t + e, in log2 units, -inf where there is no row.  The reference value `m` the
+// weights are relative to follows the maximum only when a score exceeds it by more than 8 (weights up to 2^8 cost
+// nothing in fp32), so that a tile normally needs one vote and no reduction; the same columns of o are heads 2t + e.
+// On return x holds the weights.
 template <int NT>
-__device__ __forceinline__ void rescale(float (&o)[NT][4], float alpha, int t) {
-    if (!__any_sync(0xFFFFFFFFu, alpha != 1.0f)) return;   // the maximum rarely moves after the first tiles
-    const float a0 = __shfl_sync(0xFFFFFFFFu, alpha, 8 * t), a1 = __shfl_sync(0xFFFFFFFFu, alpha, 8 * t + 4);
+__device__ __forceinline__ void softmax_step(float (&x)[4], float (&m)[2], float (&l)[2], float (&o)[NT][4]) {
+    const float top[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
+    if (__any_sync(0xFFFFFFFFu, top[0] > m[0] + 8.0f || top[1] > m[1] + 8.0f)) {
 #pragma unroll
-    for (int i = 0; i < NT; i++) { o[i][0] *= a0; o[i][1] *= a1; o[i][2] *= a0; o[i][3] *= a1; }
+        for (int e = 0; e < 2; e++) {
+            float mx = fmaxf(top[e], m[e]);
+            mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16));
+            const float alpha = mx == m[e] ? 1.0f : exp2_fast(m[e] - mx);   // 0 where nothing was seen before
+            m[e] = mx;
+            l[e] *= alpha;
+#pragma unroll
+            for (int i = 0; i < NT; i++) { o[i][e] *= alpha; o[i][2 + e] *= alpha; }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        const float ref = m[e] == -INFINITY ? 0.0f : m[e];   // nothing seen yet: every weight is 2^-inf = 0
+        x[e] = exp2_fast(x[e] - ref);
+        x[2 + e] = exp2_fast(x[2 + e] - ref);
+        l[e] += x[e] + x[2 + e];
+    }
 }
 
-// One warp's share of a tile of store rows, as loaded: lane (g, t) holds its part of the keys of rows
-// 4 (g / 2) + 2 blk + g % 2 (blk = 0, 1) and of the values and scales of rows 4t .. 4t + 3.
-template <int D>
-struct StoreTile {
-    uint32_t k[2][D / 32], v[4][D / 64], ks[4][D / 64], vs[4][D / 64];
-    uint32_t ok;                     // bit i: row 4t + i is attended (tiles that may lack rows only)
-};
+// Weights (rows of the first product's output by heads) to the layout of the second product's B operand: lane (g, t) gets
+// y[2 * blk + e] = the weight of row 4t + 2 blk + e for head g.  Row r of a block lives in the lanes of g = r.
+__device__ __forceinline__ void transpose_weights(const float (&x)[4], float (&y)[4], int g, int t) {
+#pragma unroll
+    for (int blk = 0; blk < 2; blk++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int from = 4 * (2 * t + e) + (g >> 1);
+            const float even = __shfl_sync(0xFFFFFFFFu, x[2 * blk], from), odd = __shfl_sync(0xFFFFFFFFu, x[2 * blk + 1], from);
+            y[2 * blk + e] = g & 1 ? odd : even;
+        }
+}
 
 // grid = (n_split, n_prob, ceil(group / 8)).
 //
@@ -171,12 +236,12 @@ struct StoreTile {
 // depends on (row, group) only, so it multiplies the weight, which then enters as a bf16 value and its remainder
 // (16 bits).  With at most four heads value and remainder are two column groups of ONE MMA (columns h and h + 4),
 // otherwise two MMAs.  The rows of a tile are numbered so that a lane's rows in both fragments are 4t .. 4t + 3.
-// All operands go from global memory straight to registers (the stored order of the codes makes every lane's share
-// contiguous), one tile ahead of the arithmetic; warps are independent until the end.
+// Every warp streams its tiles through a ring of its own in shared memory, three tiles ahead of the arithmetic; the stored
+// order of the codes makes each lane's share of a row one load.  Warps are independent until the end.
 //
 // 16-bit rows (resident rows, new token): the same two products on the element type, by CTAs of their own.
 template <int DT, int D, bool FEW, bool IDS>
-__global__ void __launch_bounds__(kThreads, D <= 128 ? 3 : 2)
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(D))
 q4_attend_kernel(const Args a) {
     pdl_launch_dependents();
     pdl_wait();
@@ -191,7 +256,8 @@ q4_attend_kernel(const Args a) {
     const int b = static_cast<int>(prob / a.kv_heads), h = static_cast<int>(prob % a.kv_heads);
 
     __shared__ __align__(16) uint16_t s_q[kHeads][D];
-    __shared__ __align__(16) float s_o[kWarps][kHeads][D + 4];
+    extern __shared__ __align__(128) unsigned char s_ring[];   // the warps' rings; at the end their partial outputs
+    __shared__ uint32_t s_ok[kWarps][Ring<D>::STAGES];         // rows of a tile that exist (id lists)
     __shared__ float s_ml[kWarps][kHeads][2];
     {
         const uint16_t* qb = a.q_stride_b ? a.q + b * a.q_stride_b + (static_cast<int64_t>(h) * a.group + g0) * D
@@ -210,7 +276,7 @@ q4_attend_kernel(const Args a) {
 
     const uint32_t keep_lo = FEW && g < 4 ? 0x4444u : 0x1044u, keep_hi = FEW && g < 4 ? 0x4444u : 0x3244u;
 
-    float m = -INFINITY, l = 0.0f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
     float o[NT][4];
 #pragma unroll
     for (int i = 0; i < NT; i++) { o[i][0] = 0.0f; o[i][1] = 0.0f; o[i][2] = 0.0f; o[i][3] = 0.0f; }
@@ -226,10 +292,9 @@ q4_attend_kernel(const Args a) {
         int64_t per = (n_store + a.n_store_split - 1) / a.n_store_split;
         per = (per + kTile - 1) / kTile * kTile;
         const int64_t j0 = min(n_store, split * per), j1 = min(n_store, j0 + per);
-        const uint8_t* kc = a.st.k.codes + prob * a.st.prob_rows * (D / 2) + t * (D / 8);
-        const uint8_t* vc = a.st.v.codes + prob * a.st.prob_rows * (D / 2) + g * (D / 16);
-        const uint16_t* ks = a.st.k.scales + prob * a.st.prob_rows * NG;
-        const uint16_t* vs = a.st.v.scales + prob * a.st.prob_rows * NG;
+        const uint8_t* kc = a.st.k.codes + prob * a.st.prob_rows * (D / 2);
+        const uint8_t* vc = a.st.v.codes + prob * a.st.prob_rows * (D / 2);
+        const uint8_t* sc_base = reinterpret_cast<const uint8_t*>((lane < 16 ? a.st.k.scales : a.st.v.scales) + prob * a.st.prob_rows * NG);
 
         // query fragments, normalised to [2^14, 2^15) by a power of two
         float top = 0.0f;
@@ -239,7 +304,8 @@ q4_attend_kernel(const Args a) {
         int ex = static_cast<int>((__float_as_uint(top) >> 23) & 255u);   // 0: zero or subnormal, 255: infinite
         ex = ex == 255 ? 127 + 14 : max(ex, 28);
         const float down = __uint_as_float(static_cast<uint32_t>(127 + 14 - ex + 127) << 23);   // 2^(14 - e)
-        const float up = __uint_as_float(static_cast<uint32_t>(ex - 14) << 23) * a.scale_log2;    // 2^(e - 14)
+        const float up_g = __uint_as_float(static_cast<uint32_t>(ex - 14) << 23) * a.scale_log2;  // 2^(e - 14)
+        const float up[2] = {__shfl_sync(0xFFFFFFFFu, up_g, 8 * t), __shfl_sync(0xFFFFFFFFu, up_g, 8 * t + 4)};   // heads 2t, 2t + 1
         uint32_t qa[NT][2];
 #pragma unroll
         for (int w = 0; w < D / 64; w++)
@@ -254,101 +320,154 @@ q4_attend_kernel(const Args a) {
                                                                  elem_to_float<DT>(qrow[d + 16 + e]) * down);
                 }
 
-        // A whole tile of consecutive rows: every address is a lane constant plus the first row.
-        auto load_run = [&](StoreTile<D>& x, int64_t row0) {
-            const uint8_t* kp = kc + (row0 + 4 * (g >> 1) + (g & 1)) * (D / 2);
-            const uint8_t* vp = vc + (row0 + 4 * t) * (D / 2);
-            const uint16_t* ksp = ks + (row0 + 4 * t) * NG;
-            const uint16_t* vsp = vs + (row0 + 4 * t) * NG;
-            load_words<D / 32>(x.k[0], kp);
-            load_words<D / 32>(x.k[1], kp + D);
+        // ---- the ring: lane copies chunks lane + 32 j of both tensors' codes and one row's scales of one tensor ----
+        using R = Ring<D>;
+        constexpr int CPR = D / 32;                    // chunks per row
+        constexpr int NC = kTile * CPR / 32;           // chunks per lane and tensor
+        const unsigned ring = smem_u32(s_ring) + warp * R::STAGES * R::STAGE;
+        int dst[NC];
 #pragma unroll
-            for (int i = 0; i < 4; i++) load_words<D / 64>(x.ks[i], ksp + i * NG);
-#pragma unroll
-            for (int i = 0; i < 4; i++) load_words<D / 64>(x.v[i], vp + i * (D / 2));
-#pragma unroll
-            for (int i = 0; i < 4; i++) load_words<D / 64>(x.vs[i], vsp + i * NG);
-        };
+        for (int j = 0; j < NC; j++) dst[j] = R::chunk((lane + 32 * j) / CPR, (lane + 32 * j) % CPR);
+        const int dst_scale = 2 * R::CODES + lane * (D / 16);
         // This lane's row of a tile's 16 (lane and lane + 16 hold the same); -1 where there is none.
-        auto fetch_id = [&](int64_t base) -> int32_t {
-            const int64_t j = base + (lane & 15);
+        auto fetch_id = [&](int i) -> int32_t {
+            const int64_t j = j0 + (warp + static_cast<int64_t>(i) * kWarps) * kTile + (lane & 15);
             if (j >= j1) return -1;
-            if (!IDS) return static_cast<int32_t>(j);
             const int64_t row = static_cast<int64_t>(sel[j]) - a.sel_base;
             return row >= 0 && row < n_rows ? static_cast<int32_t>(row) : -1;   // pads and ids of other shards
         };
-        // Any 16 rows; where there is none, row 0 (which exists) is loaded and not used.
-        auto load_any = [&](StoreTile<D>& x, int32_t id) {
-            const int32_t safe = max(id, 0);
-            x.ok = (__ballot_sync(0xFFFFFFFFu, id >= 0) >> (4 * t)) & 15u;
+        // Consecutive rows: 16 of them are one run of bytes per array, so the addresses just advance from tile to tile.
+        const uint8_t* kp = kc + (j0 + warp * kTile) * (D / 2) + lane * 16;
+        const uint8_t* vp = vc + (j0 + warp * kTile) * (D / 2) + lane * 16;
+        const uint8_t* sp = sc_base + (j0 + warp * kTile + (lane & 15)) * (D / 16);
+        const int n_mine = static_cast<int>((max(j1 - j0 - warp * kTile, static_cast<int64_t>(0)) + kWarps * kTile - 1) / (kWarps * kTile));
+        const int last_rows = static_cast<int>(j1 - j0) - (warp + (n_mine - 1) * kWarps) * kTile;   // of this warp's last tile; > 16: whole
+        auto issue = [&](unsigned st, int i, int32_t id) {   // this warp's tile i into the stage at st
+            if (!IDS) {
+                if (i < n_mine - 1 || (i == n_mine - 1 && last_rows >= kTile)) {
 #pragma unroll
-            for (int blk = 0; blk < 2; blk++) {
-                const int64_t row = __shfl_sync(0xFFFFFFFFu, safe, 4 * (g >> 1) + 2 * blk + (g & 1));
-                load_words<D / 32>(x.k[blk], kc + row * (D / 2));
-            }
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int64_t row = __shfl_sync(0xFFFFFFFFu, safe, 4 * t + i);
-                load_words<D / 64>(x.ks[i], ks + row * NG);
-                load_words<D / 64>(x.v[i], vc + row * (D / 2));
-                load_words<D / 64>(x.vs[i], vs + row * NG);
-            }
-        };
-        auto compute = [&](StoreTile<D>& x, bool whole) {
-            float sc[4];
-#pragma unroll
-            for (int blk = 0; blk < 2; blk++) {
-                float acc[NG][4];
-#pragma unroll
-                for (int i = 0; i < NG; i++) { acc[i][0] = 0.0f; acc[i][1] = 0.0f; acc[i][2] = 0.0f; acc[i][3] = 0.0f; }
-#pragma unroll
-                for (int c = 0; c < 2; c++)
-#pragma unroll
-                    for (int w = 0; w < D / 64; w++) {
-                        uint32_t p[4];
-                        codes_f16(x.k[blk][c * (D / 64) + w], p);
-                        mma<false>(acc[2 * w], qa[4 * w + c][0], 0u, qa[4 * w + c][1], 0u, p[0], p[1]);
-                        mma<false>(acc[2 * w + 1], qa[4 * w + 2 + c][0], 0u, qa[4 * w + 2 + c][1], 0u, p[2], p[3]);
+                    for (int j = 0; j < NC; j++) {
+                        copy_async<16>(st + dst[j], kp + 512 * j);
+                        copy_async<16>(st + R::CODES + dst[j], vp + 512 * j);
                     }
+                    copy_async<D / 16>(st + dst_scale, sp);
+                } else if (i < n_mine) {               // the last rows; zeros behind them
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    float s = 0.0f;
-#pragma unroll
-                    for (int w = 0; w < D / 64; w++) {
-                        s = fmaf(low_elem<DT>(x.ks[2 * blk + e][w]), acc[2 * w][e], s);
-                        s = fmaf(high_elem<DT>(x.ks[2 * blk + e][w]), acc[2 * w + 1][e], s);
+                    for (int j = 0; j < NC; j++) {
+                        const bool ok = (lane + 32 * j) / CPR < last_rows;
+                        copy_async<16>(st + dst[j], ok ? kp + 512 * j : kc, ok);
+                        copy_async<16>(st + R::CODES + dst[j], ok ? vp + 512 * j : vc, ok);
                     }
-                    sc[2 * blk + e] = s * up;
+                    const bool ok = (lane & 15) < last_rows;
+                    copy_async<D / 16>(st + dst_scale, ok ? sp : sc_base, ok);
                 }
+                kp += kWarps * kTile * (D / 2);
+                vp += kWarps * kTile * (D / 2);
+                sp += kWarps * kTile * (D / 16);
+            } else {
+#pragma unroll
+                for (int j = 0; j < NC; j++) {
+                    const int32_t row = __shfl_sync(0xFFFFFFFFu, id, (lane + 32 * j) / CPR);
+                    const int64_t off = max(row, 0) * static_cast<int64_t>(D / 2) + (lane + 32 * j) % CPR * 16;
+                    copy_async<16>(st + dst[j], kc + off, row >= 0);
+                    copy_async<16>(st + R::CODES + dst[j], vc + off, row >= 0);
+                }
+                copy_async<D / 16>(st + dst_scale, sc_base + max(id, 0) * static_cast<int64_t>(D / 16), id >= 0);
+                const uint32_t ok = __ballot_sync(0xFFFFFFFFu, id >= 0) & 0xFFFFu;
+                if (lane == 0) s_ok[warp][i % R::STAGES] = ok;
             }
-            if (!whole) {   // rows that are not there: no weight, and a scale of 0 in place of whatever was loaded
+            copy_commit();
+        };
+        // where this lane reads: keys of rows 4 (g / 2) + 2 blk + g % 2, values and scales of rows 4t + i
+        unsigned k_at[2], v_at[4];
+        const unsigned ks_at = 2 * R::CODES + (4 * (g >> 1) + (g & 1)) * (D / 16);
+#pragma unroll
+        for (int blk = 0; blk < 2; blk++) {
+            const int r = 4 * (g >> 1) + 2 * blk + (g & 1);
+            k_at[blk] = D == 64 ? R::chunk(r, t >> 1) + (t & 1) * 8 : R::chunk(r, D == 128 ? t : 2 * t);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            v_at[i] = R::CODES + R::chunk(4 * t + i, g * (D / 16) / 16) + g * (D / 16) % 16;
+        auto compute = [&](unsigned st, uint32_t ok) {
+            float sc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            {
+                uint32_t kw[2][D / 32], ks[2][D / 64];
+#pragma unroll
+                for (int blk = 0; blk < 2; blk++) {
+                    if (D == 256) {                    // chunks 2t and 2t + 1: the permutation flips bit 0 or not
+                        uint32_t half[4];
+                        lds_words<4>(half, st + k_at[blk]);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) kw[blk][i] = half[i];
+                        lds_words<4>(half, st + (k_at[blk] ^ 16u));
+#pragma unroll
+                        for (int i = 0; i < 4; i++) kw[blk][(D / 64 + i) % (D / 32)] = half[i];
+                    } else {
+                        lds_words<D / 32>(kw[blk], st + k_at[blk]);
+                    }
+                    lds_words<D / 64>(ks[blk], st + ks_at + 2 * blk * (D / 16));
+                }
+#pragma unroll
+                for (int w = 0; w < D / 64; w++) {
+                    float acc[2][4];
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        uint32_t p[4], r[4];
+                        codes_f16(kw[0][c * (D / 64) + w], p);
+                        codes_f16(kw[1][c * (D / 64) + w], r);
+#pragma unroll
+                        for (int gp = 0; gp < 2; gp++) {
+                            const uint32_t (&q)[2] = qa[4 * w + 2 * gp + c];
+                            if (c == 0) mma_first<false>(acc[gp], p[2 * gp], r[2 * gp], p[2 * gp + 1], r[2 * gp + 1], q[0], q[1]);
+                            else mma<false>(acc[gp], p[2 * gp], r[2 * gp], p[2 * gp + 1], r[2 * gp + 1], q[0], q[1]);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        sc[i] = fmaf(low_elem<DT>(ks[i >> 1][w]), acc[0][i], sc[i]);
+                        sc[i] = fmaf(high_elem<DT>(ks[i >> 1][w]), acc[1][i], sc[i]);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) sc[i] *= up[i & 1];
+            }
+            if (ok != 0xFFFFu) {   // rows that are not there: no weight (their scales and codes are zeros)
+                const int r = 4 * (g >> 1) + (g & 1);
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    if (((x.ok >> i) & 1u) == 0) {
-                        sc[i] = -INFINITY;
-#pragma unroll
-                        for (int w = 0; w < D / 64; w++) x.vs[i][w] = 0;
-                    }
+                    if (((ok >> (r + 2 * (i >> 1))) & 1u) == 0) sc[i] = -INFINITY;
             }
-            rescale<NT>(o, softmax_step(sc, m, l), t);
+            softmax_step<NT>(sc, m, l, o);
+            float wt[4];
+            transpose_weights(sc, wt, g, t);
+            constexpr int WV = D == 64 ? 1 : 2;        // words of a row's values and scales read at a time
+            uint32_t vw[4][WV], vs[4][WV];
 #pragma unroll
             for (int w = 0; w < D / 64; w++) {
+                if (w % WV == 0) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        lds_words<WV>(vw[i], st + v_at[i] + 4 * w);
+                        lds_words<WV>(vs[i], st + 2 * R::CODES + R::SCALES + (4 * t + i) * (D / 16) + 4 * w);
+                    }
+                }
                 uint32_t hi[2][2], lo[2][2];   // [group of the word][row block]
 #pragma unroll
                 for (int gp = 0; gp < 2; gp++)
 #pragma unroll
                     for (int blk = 0; blk < 2; blk++) {
-                        const float p0 = sc[2 * blk] * (gp ? high_elem<DT>(x.vs[2 * blk][w]) : low_elem<DT>(x.vs[2 * blk][w]));
-                        const float p1 = sc[2 * blk + 1] *
-                                         (gp ? high_elem<DT>(x.vs[2 * blk + 1][w]) : low_elem<DT>(x.vs[2 * blk + 1][w]));
+                        const float p0 = wt[2 * blk] * (gp ? high_elem<DT>(vs[2 * blk][w % WV]) : low_elem<DT>(vs[2 * blk][w % WV]));
+                        const float p1 = wt[2 * blk + 1] *
+                                         (gp ? high_elem<DT>(vs[2 * blk + 1][w % WV]) : low_elem<DT>(vs[2 * blk + 1][w % WV]));
                         split_pair<true, FEW>(p0, p1, keep_lo, keep_hi, hi[gp][blk], lo[gp][blk]);
                     }
                 // value codes of rows (4t, 4t + 1) and (4t + 2, 4t + 3): nibble pairs of the same element
                 uint32_t va[2][2][4];
 #pragma unroll
                 for (int blk = 0; blk < 2; blk++) {
-                    codes_bf16(__byte_perm(x.v[2 * blk][w], x.v[2 * blk + 1][w], 0x5410), va[blk][0]);   // tiles 4w, 4w + 2
-                    codes_bf16(__byte_perm(x.v[2 * blk][w], x.v[2 * blk + 1][w], 0x7632), va[blk][1]);   // tiles 4w + 1, 4w + 3
+                    codes_bf16(__byte_perm(vw[2 * blk][w % WV], vw[2 * blk + 1][w % WV], 0x5410), va[blk][0]);   // tiles 4w, 4w + 2
+                    codes_bf16(__byte_perm(vw[2 * blk][w % WV], vw[2 * blk + 1][w % WV], 0x7632), va[blk][1]);   // tiles 4w + 1, 4w + 3
                 }
 #pragma unroll
                 for (int tile = 0; tile < 4; tile++) {
@@ -365,49 +484,25 @@ q4_attend_kernel(const Args a) {
                     }
             }
         };
-        const int64_t step = kWarps * kTile;
-        int64_t base = j0 + warp * kTile;
-        if (!IDS) {
-            if (D <= 128 && base + kTile <= j1) {      // one tile ahead, in two sets of registers
-                StoreTile<D> x, y;
-                load_run(x, base);
-                while (true) {
-                    if (base + step + kTile > j1) { compute(x, true); base += step; break; }
-                    load_run(y, base + step);
-                    compute(x, true);
-                    base += step;
-                    if (base + step + kTile > j1) { compute(y, true); base += step; break; }
-                    load_run(x, base + step);
-                    compute(y, true);
-                    base += step;
-                }
-            }
-            StoreTile<D> x;
-            for (; base < j1; base += step) {          // the last tile; every tile where registers do not hold two
-                const bool whole = base + kTile <= j1;
-                if (whole) load_run(x, base);
-                else load_any(x, fetch_id(base));
-                compute(x, whole);
-            }
-        } else if (base < j1) {
-            StoreTile<D> x, y;
-            load_any(x, fetch_id(base));
-            int32_t id = fetch_id(base + step);
-            while (true) {
-                bool more = base + step < j1;
-                if (D <= 128 && more) { load_any(y, id); id = fetch_id(base + 2 * step); }
-                compute(x, __all_sync(0xFFFFFFFFu, x.ok == 15u));
-                if (!more) break;
-                base += step;
-                more = base + step < j1;
-                if (D > 128) { load_any(y, id); id = fetch_id(base + step); }
-                else if (more) { load_any(x, id); id = fetch_id(base + 2 * step); }
-                compute(y, __all_sync(0xFFFFFFFFu, y.ok == 15u));
-                if (!more) break;
-                base += step;
-                if (D > 128) { load_any(x, id); id = fetch_id(base + step); }
+        int32_t id = IDS ? fetch_id(0) : 0;
+        if (n_mine > 0) {
+#pragma unroll
+            for (int i = 0; i < R::STAGES - 1; i++) {  // tiles beyond the last copy nothing
+                issue(ring + i * R::STAGE, i, id);
+                if (IDS) id = fetch_id(i + 1);
             }
         }
+        unsigned now = ring, next = ring + (R::STAGES - 1) * R::STAGE;
+        for (int i = 0; i < n_mine; i++) {
+            copy_wait<R::STAGES - 2>();
+            __syncwarp();   // every lane's copies of this tile have landed, and nobody reads the tile before any more
+            issue(next, i + R::STAGES - 1, id);
+            if (IDS) id = fetch_id(i + R::STAGES);
+            compute(now, IDS ? s_ok[warp][i % R::STAGES] : i < n_mine - 1 || last_rows >= kTile ? 0xFFFFu : (1u << last_rows) - 1u);
+            next = now;
+            now = now == ring + (R::STAGES - 1) * R::STAGE ? ring : now + R::STAGE;
+        }
+        copy_wait<0>();
     } else {
         // flash-attn's in-place append of the new token (base.py:134-142): one CTA per problem
         if (has_new && split == a.n_store_split && blockIdx.z == 0 && a.res_k != nullptr && tid < D / 8) {
@@ -430,27 +525,18 @@ q4_attend_kernel(const Args a) {
             return j < res_len ? res + res_off + static_cast<int64_t>(j) * D : fresh + new_off;
         };
         for (int base = j0 + warp * kTile; base < j1; base += kWarps * kTile) {
-            float sc[4];
+            uint4 kw[2][D / 32];
+            int row[2];
 #pragma unroll
             for (int blk = 0; blk < 2; blk++) {
-                const int j = base + 4 * (g >> 1) + 2 * blk + (g & 1);
-                uint4 kw[D / 32];
+                row[blk] = base + 4 * (g >> 1) + 2 * blk + (g & 1);
 #pragma unroll
-                for (int i = 0; i < D / 32; i++) kw[i] = make_uint4(0, 0, 0, 0);
-                if (j < j1) {
-                    const uint16_t* kp = row_ptr(a.res_k, a.k_new, j) + 8 * t;
+                for (int i = 0; i < D / 32; i++) kw[blk][i] = make_uint4(0, 0, 0, 0);
+                if (row[blk] < j1) {
+                    const uint16_t* kp = row_ptr(a.res_k, a.k_new, row[blk]) + 8 * t;
 #pragma unroll
-                    for (int i = 0; i < D / 32; i++) kw[i] = *reinterpret_cast<const uint4*>(kp + 32 * i);
+                    for (int i = 0; i < D / 32; i++) kw[blk][i] = *reinterpret_cast<const uint4*>(kp + 32 * i);
                 }
-                float acc[2][4] = {};
-#pragma unroll
-                for (int i = 0; i < D / 32; i++) {
-                    mma<BF16>(acc[0], qa[2 * i][0], 0u, qa[2 * i][1], 0u, kw[i].x, kw[i].y);
-                    mma<BF16>(acc[1], qa[2 * i + 1][0], 0u, qa[2 * i + 1][1], 0u, kw[i].z, kw[i].w);
-                }
-#pragma unroll
-                for (int e = 0; e < 2; e++)
-                    sc[2 * blk + e] = base + 4 * t + 2 * blk + e < j1 ? (acc[0][e] + acc[1][e]) * a.scale_log2 : -INFINITY;
             }
             uint32_t vw[4][NT];              // rows 4t .. 4t + 3, elements g * D / 8 .. + D / 8
 #pragma unroll
@@ -467,11 +553,26 @@ q4_attend_kernel(const Args a) {
                     }
                 }
             }
-            rescale<NT>(o, softmax_step(sc, m, l), t);
+            float acc[2][4];
+#pragma unroll
+            for (int i = 0; i < D / 32; i++) {
+                if (i == 0) {
+                    mma_first<BF16>(acc[0], kw[0][i].x, kw[1][i].x, kw[0][i].y, kw[1][i].y, qa[2 * i][0], qa[2 * i][1]);
+                    mma_first<BF16>(acc[1], kw[0][i].z, kw[1][i].z, kw[0][i].w, kw[1][i].w, qa[2 * i + 1][0], qa[2 * i + 1][1]);
+                } else {
+                    mma<BF16>(acc[0], kw[0][i].x, kw[1][i].x, kw[0][i].y, kw[1][i].y, qa[2 * i][0], qa[2 * i][1]);
+                    mma<BF16>(acc[1], kw[0][i].z, kw[1][i].z, kw[0][i].w, kw[1][i].w, qa[2 * i + 1][0], qa[2 * i + 1][1]);
+                }
+            }
+            float sc[4], wt[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) sc[i] = row[i >> 1] < j1 ? (acc[0][i] + acc[1][i]) * a.scale_log2 : -INFINITY;
+            softmax_step<NT>(sc, m, l, o);
+            transpose_weights(sc, wt, g, t);
             uint32_t hi[2], lo[2];
 #pragma unroll
             for (int blk = 0; blk < 2; blk++) {
-                split_pair<BF16, FEW>(sc[2 * blk], sc[2 * blk + 1], keep_lo, keep_hi, hi[blk], lo[blk]);
+                split_pair<BF16, FEW>(wt[2 * blk], wt[2 * blk + 1], keep_lo, keep_hi, hi[blk], lo[blk]);
             }
 #pragma unroll
             for (int n = 0; n < NT; n++) {
@@ -484,9 +585,14 @@ q4_attend_kernel(const Args a) {
     }
 
     // ---- merge the warps (log-sum-exp) and write this split's partial ----
-    l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
-    l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
-    if (t == 0) { s_ml[warp][g][0] = m; s_ml[warp][g][1] = l; }
+    __syncthreads();   // the rings are idle: they hold the warps' outputs now
+    float (*s_o)[kHeads][D + 4] = reinterpret_cast<float (*)[kHeads][D + 4]>(s_ring);
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+#pragma unroll
+        for (int off = 4; off <= 16; off <<= 1) l[e] += __shfl_xor_sync(0xFFFFFFFFu, l[e], off);
+        if (g == 0) { s_ml[warp][2 * t + e][0] = m[e]; s_ml[warp][2 * t + e][1] = l[e]; }
+    }
 #pragma unroll
     for (int i = 0; i < NT; i++) {
         if (FEW)   // columns h and h + 4 are the two halves of head h's weights
@@ -518,15 +624,33 @@ q4_attend_kernel(const Args a) {
     }
 }
 
-// CTAs per problem (and chunk of 8 heads).  One wave of three CTAs per SM; a 16-bit row counts as three store rows (its
+// CTAs per problem (and chunk of 8 heads).  One wave of the CTAs that fit an SM; a 16-bit row counts as three store rows (its
 // 512 bytes at head_dim 128 against 144); every kind of row that occurs gets at least one CTA.
-constexpr int kCtasPerSm = 3;
 constexpr int kMaxSplits = 256;
+
+template <int DT, int D, bool FEW, bool IDS>
+int launch_one(const Args& a, dim3 grid, cudaStream_t stream) {
+    static PerDeviceOnce once;   // > 48 KB of dynamic shared memory needs an opt-in per kernel and device
+    int rc = once.run([](int) {
+        DC_CUDA_TRY(cudaFuncSetAttribute(q4_attend_kernel<DT, D, FEW, IDS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(attend_smem_bytes<D>())));
+        return DC_OK;
+    });
+    if (rc != DC_OK) return rc;
+    DC_CUDA_TRY(launch_chained(q4_attend_kernel<DT, D, FEW, IDS>, grid, dim3(kThreads), attend_smem_bytes<D>(), stream, 0u, a));
+    return DC_OK;
+}
+
+template <int DT, int D>
+int launch(const Args& a, bool few, bool ids, dim3 grid, cudaStream_t stream) {
+    if (few) return ids ? launch_one<DT, D, true, true>(a, grid, stream) : launch_one<DT, D, true, false>(a, grid, stream);
+    return ids ? launch_one<DT, D, false, true>(a, grid, stream) : launch_one<DT, D, false, false>(a, grid, stream);
+}
 
 struct Split { int store, total; };
 
-Split splits(int n_prob, int64_t store_rows, int64_t res_rows) {
-    const int64_t target = std::max(1, kCtasPerSm * sm_count() / std::max(1, n_prob));
+Split splits(int n_prob, int head_dim, int64_t store_rows, int64_t res_rows) {
+    const int64_t target = std::max(1, ctas_per_sm(head_dim) * sm_count() / std::max(1, n_prob));
     const int64_t w_store = (store_rows + 63) / 64, w_res = (3 * res_rows + 63) / 64;   // units of 64 store rows
     const int64_t total = std::max<int64_t>(1, std::min<int64_t>(std::min(target, w_store + w_res), kMaxSplits - 1));
     int64_t store = 0, res = 0;
@@ -541,9 +665,9 @@ Split splits(int n_prob, int64_t store_rows, int64_t res_rows) {
 }  // namespace
 
 int64_t q4_attend_scratch_bytes(int n_prob, int group, int head_dim) {
-    // splits() makes at most kCtasPerSm * SMs / n_prob + 1 per problem (2 where that is 0 or 1), and at most kMaxSplits
+    // splits() makes at most ctas_per_sm * SMs / n_prob + 1 per problem (2 where that is 0 or 1), and at most kMaxSplits
     const int64_t ctas = std::min<int64_t>(static_cast<int64_t>(n_prob) * kMaxSplits,
-                                           static_cast<int64_t>(kCtasPerSm) * sm_count() + 2ll * n_prob);
+                                           static_cast<int64_t>(ctas_per_sm(head_dim)) * sm_count() + 2ll * n_prob);
     return ctas * group * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
 }
 
@@ -580,17 +704,15 @@ int q4_attend(const Q4Attend& in, cudaStream_t stream) {
     a.res_stride_b = in.res_stride_b; a.res_stride_h = in.res_stride_h;
     a.res_len = in.res_len; a.res_len_dev = in.res_len_dev;
     a.scale_log2 = (in.scale > 0.0f ? in.scale : 1.0f / std::sqrt(static_cast<float>(in.head_dim))) * kLog2e;
-    const Split sp = splits(in.n_prob, in.n_sel < 0 ? in.n_rows : in.n_sel, in.res_len + (in.k_new ? 1 : 0));
+    const Split sp = splits(in.n_prob, in.head_dim, in.n_sel < 0 ? in.n_rows : in.n_sel, in.res_len + (in.k_new ? 1 : 0));
     a.n_store_split = sp.store;
     a.n_split = sp.total;
     a.part_acc = static_cast<float*>(in.scratch);
     a.part_ml = a.part_acc + static_cast<int64_t>(in.n_prob) * a.n_split * in.group * in.head_dim;
     const dim3 grid(static_cast<unsigned>(a.n_split), static_cast<unsigned>(in.n_prob),
                     static_cast<unsigned>((in.group + kHeads - 1) / kHeads));
-#define LAUNCH(DT, D, FEW, IDS) DC_CUDA_TRY(launch_chained(q4_attend_kernel<DT, D, FEW, IDS>, grid, dim3(kThreads), 0, stream, 0u, a))
-#define CASE(DT, D)                                                                                   \
-    if (in.group <= 4) { if (in.n_sel < 0) LAUNCH(DT, D, true, false); else LAUNCH(DT, D, true, true); } \
-    else { if (in.n_sel < 0) LAUNCH(DT, D, false, false); else LAUNCH(DT, D, false, true); }
+#define CASE(DT, D) rc = launch<DT, D>(a, in.group <= 4, in.n_sel >= 0, grid, stream)
+    int rc = DC_OK;
     if (in.dtype == DC_BF16) {
         if (in.head_dim == 64) { CASE(DC_BF16, 64); }
         else if (in.head_dim == 128) { CASE(DC_BF16, 128); }
@@ -601,7 +723,7 @@ int q4_attend(const Q4Attend& in, cudaStream_t stream) {
         else { CASE(DC_FP16, 256); }
     }
 #undef CASE
-#undef LAUNCH
+    if (rc != DC_OK) return rc;
     return lse_combine(a.part_acc, in.head_dim, static_cast<int64_t>(a.n_split) * in.head_dim, a.part_ml, 2,
                        static_cast<int64_t>(a.n_split) * 2, a.n_split, static_cast<int64_t>(in.n_prob) * in.group, in.head_dim,
                        in.dtype, in.out, in.out_lse, in.out_acc, in.out_ml, stream, nullptr, in.xout, in.fin, true);
