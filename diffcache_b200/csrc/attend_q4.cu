@@ -20,13 +20,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kHeads = 8;            // query heads of one kv head handled by one CTA (columns of the second product)
 constexpr int kTile = 16;            // rows a warp takes at a time
 constexpr float kLog2e = 1.4426950408889634f;
-#ifndef Q4_C
-#define Q4_C 3
-#endif
-#ifndef Q4_S
-#define Q4_S 4
-#endif
-__host__ __device__ constexpr int ctas_per_sm(int head_dim) { return head_dim <= 128 ? Q4_C : 2; }
+__host__ __device__ constexpr int ctas_per_sm(int head_dim) { return head_dim <= 128 ? 4 : 2; }
 
 struct Args {
     Q4Store st;
@@ -111,7 +105,7 @@ struct Ring {
     static constexpr int CODES = kTile * (D / 2);        // one tensor's codes of a tile
     static constexpr int SCALES = kTile * (D / 16);
     static constexpr int STAGE = 2 * CODES + 2 * SCALES; // [K codes | V codes | K scales | V scales]
-    static constexpr int STAGES = Q4_S;
+    static constexpr int STAGES = 4;
     // Byte of 16-byte chunk c of row r among a tile's codes.  Rows and chunks are permuted so that neither the keys (eight
     // rows, a quarter row per lane) nor the values (rows 4t + i, an eighth per lane) make a warp's lanes share banks.
     __device__ static __forceinline__ int chunk(int r, int c) {
@@ -127,22 +121,36 @@ constexpr size_t attend_smem_bytes() {
     return ring > merge ? ring : merge;
 }
 
+// Constants of the code conversion, kept in registers: with an immediate operand the packed 16-bit subtraction issues to
+// the integer pipe, which the masks already fill, instead of the FMA pipe.
+struct CodeConst {
+    uint32_t f16_one, f16_off, f16_16th, f16_off16, bf16_one, bf16_off;
+    __device__ __forceinline__ explicit CodeConst(uint32_t zero) {   // 0, in a form the compiler cannot fold
+        f16_one = 0x64006400u | zero;    // 1024, 1024
+        f16_off = 0xE408E408u | zero;    // -1032
+        f16_16th = 0x2C002C00u | zero;   // 1 / 16
+        f16_off16 = 0xD480D480u | zero;  // -72
+        bf16_one = 0x43004300u | zero;   // 128, 128
+        bf16_off = 0xC308C308u | zero;   // -136
+    }
+};
+
 // Four pairs of codes of a word: pair j = (nibble j, nibble j + 4).  Inserting a nibble into the mantissa of 1024 (fp16) or
 // 128 (bf16) makes it that number plus the nibble, exactly; the offset and the 8 of the encoding go with one operation.
-__device__ __forceinline__ void codes_f16(uint32_t w, uint32_t (&p)[4]) {
+__device__ __forceinline__ void codes_f16(const CodeConst& k, uint32_t w, uint32_t (&p)[4]) {
     const uint32_t hi = w >> 8;
-    uint32_t t[4] = {(w & 0x000F000Fu) | 0x64006400u, (w & 0x00F000F0u) | 0x64006400u,
-                     (hi & 0x000F000Fu) | 0x64006400u, (hi & 0x00F000F0u) | 0x64006400u};
-    asm("sub.f16x2 %0, %1, %2;\n" : "=r"(p[0]) : "r"(t[0]), "r"(0x64086408u));                       // - 1032
-    asm("fma.rn.f16x2 %0, %1, %2, %3;\n" : "=r"(p[1]) : "r"(t[1]), "r"(0x2C002C00u), "r"(0xD480D480u));   // / 16 - 72
-    asm("sub.f16x2 %0, %1, %2;\n" : "=r"(p[2]) : "r"(t[2]), "r"(0x64086408u));
-    asm("fma.rn.f16x2 %0, %1, %2, %3;\n" : "=r"(p[3]) : "r"(t[3]), "r"(0x2C002C00u), "r"(0xD480D480u));
+    const uint32_t t[4] = {(w & 0x000F000Fu) | k.f16_one, (w & 0x00F000F0u) | k.f16_one, (hi & 0x000F000Fu) | k.f16_one,
+                           (hi & 0x00F000F0u) | k.f16_one};
+    asm("add.f16x2 %0, %1, %2;\n" : "=r"(p[0]) : "r"(t[0]), "r"(k.f16_off));
+    asm("fma.rn.f16x2 %0, %1, %2, %3;\n" : "=r"(p[1]) : "r"(t[1]), "r"(k.f16_16th), "r"(k.f16_off16));
+    asm("add.f16x2 %0, %1, %2;\n" : "=r"(p[2]) : "r"(t[2]), "r"(k.f16_off));
+    asm("fma.rn.f16x2 %0, %1, %2, %3;\n" : "=r"(p[3]) : "r"(t[3]), "r"(k.f16_16th), "r"(k.f16_off16));
 }
-__device__ __forceinline__ void codes_bf16(uint32_t w, uint32_t (&p)[4]) {
+__device__ __forceinline__ void codes_bf16(const CodeConst& k, uint32_t w, uint32_t (&p)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const uint32_t t = ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
-        asm("sub.bf16x2 %0, %1, %2;\n" : "=r"(p[i]) : "r"(t), "r"(0x43084308u));                      // - 136
+        const uint32_t t = ((w >> (4 * i)) & 0x000F000Fu) | k.bf16_one;
+        asm("add.bf16x2 %0, %1, %2;\n" : "=r"(p[i]) : "r"(t), "r"(k.bf16_off));
     }
 }
 
@@ -229,9 +237,9 @@ __device__ __forceinline__ void transpose_weights(const float (&x)[4], float (&y
 
 // grid = (n_split, n_prob, ceil(group / 8)).
 //
-// Store rows.  S = Q K^T with m16n8k16 MMAs: the query heads are the rows of A, 8 store rows the columns of B.  The codes
-// enter as small integers (fp16, exact), so a group's partial product is exact up to fp32 accumulation and its scale is
-// applied once, in fp32.  The query of a head is normalised by a power of two so that a bf16 query is exact in fp16 too.
+// Store rows.  S^T = K Q^T with m16n8k16 MMAs: 16 store rows are the rows of A, up to 8 query heads the columns of B.  The
+// codes enter as small integers (fp16, exact), so a group's partial product is exact up to fp32 accumulation and its scale
+// is applied once, in fp32.  The query of a head is normalised by a power of two so that a bf16 query is exact in fp16 too.
 // O^T = V^T P^T: the value codes are A (16 elements of a tile x 16 rows, bf16 integers), the weights are B; a value's scale
 // depends on (row, group) only, so it multiplies the weight, which then enters as a bf16 value and its remainder
 // (16 bits).  With at most four heads value and remainder are two column groups of ONE MMA (columns h and h + 4),
@@ -389,6 +397,7 @@ q4_attend_kernel(const Args a) {
 #pragma unroll
         for (int i = 0; i < 4; i++)
             v_at[i] = R::CODES + R::chunk(4 * t + i, g * (D / 16) / 16) + g * (D / 16) % 16;
+        const CodeConst cc(static_cast<uint32_t>(a.kv_heads) >> 31);
         auto compute = [&](unsigned st, uint32_t ok) {
             float sc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             {
@@ -414,8 +423,8 @@ q4_attend_kernel(const Args a) {
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
                         uint32_t p[4], r[4];
-                        codes_f16(kw[0][c * (D / 64) + w], p);
-                        codes_f16(kw[1][c * (D / 64) + w], r);
+                        codes_f16(cc, kw[0][c * (D / 64) + w], p);
+                        codes_f16(cc, kw[1][c * (D / 64) + w], r);
 #pragma unroll
                         for (int gp = 0; gp < 2; gp++) {
                             const uint32_t (&q)[2] = qa[4 * w + 2 * gp + c];
@@ -466,8 +475,8 @@ q4_attend_kernel(const Args a) {
                 uint32_t va[2][2][4];
 #pragma unroll
                 for (int blk = 0; blk < 2; blk++) {
-                    codes_bf16(__byte_perm(vw[2 * blk][w % WV], vw[2 * blk + 1][w % WV], 0x5410), va[blk][0]);   // tiles 4w, 4w + 2
-                    codes_bf16(__byte_perm(vw[2 * blk][w % WV], vw[2 * blk + 1][w % WV], 0x7632), va[blk][1]);   // tiles 4w + 1, 4w + 3
+                    codes_bf16(cc, __byte_perm(vw[2 * blk][w % WV], vw[2 * blk + 1][w % WV], 0x5410), va[blk][0]);   // tiles 4w, 4w + 2
+                    codes_bf16(cc, __byte_perm(vw[2 * blk][w % WV], vw[2 * blk + 1][w % WV], 0x7632), va[blk][1]);   // tiles 4w + 1, 4w + 3
                 }
 #pragma unroll
                 for (int tile = 0; tile < 4; tile++) {
@@ -624,8 +633,9 @@ q4_attend_kernel(const Args a) {
     }
 }
 
-// CTAs per problem (and chunk of 8 heads).  One wave of the CTAs that fit an SM; a 16-bit row counts as three store rows (its
-// 512 bytes at head_dim 128 against 144); every kind of row that occurs gets at least one CTA.
+// CTAs per problem (and chunk of 8 heads).  One wave of the CTAs that fit an SM; a 16-bit row costs as much as 2.7 consecutive
+// store rows or 1.6 gathered ones (115, 42 and 70 ps measured at head_dim 128); every kind of row that occurs gets at
+// least one CTA.
 constexpr int kMaxSplits = 256;
 
 template <int DT, int D, bool FEW, bool IDS>
@@ -649,9 +659,9 @@ int launch(const Args& a, bool few, bool ids, dim3 grid, cudaStream_t stream) {
 
 struct Split { int store, total; };
 
-Split splits(int n_prob, int head_dim, int64_t store_rows, int64_t res_rows) {
+Split splits(int n_prob, int head_dim, bool ids, int64_t store_rows, int64_t res_rows) {
     const int64_t target = std::max(1, ctas_per_sm(head_dim) * sm_count() / std::max(1, n_prob));
-    const int64_t w_store = (store_rows + 63) / 64, w_res = (3 * res_rows + 63) / 64;   // units of 64 store rows
+    const int64_t w_store = (store_rows + 63) / 64, w_res = ((ids ? 16 : 27) * res_rows + 639) / 640;   // units of 64 store rows
     const int64_t total = std::max<int64_t>(1, std::min<int64_t>(std::min(target, w_store + w_res), kMaxSplits - 1));
     int64_t store = 0, res = 0;
     if (w_store + w_res > 0) {
@@ -704,7 +714,7 @@ int q4_attend(const Q4Attend& in, cudaStream_t stream) {
     a.res_stride_b = in.res_stride_b; a.res_stride_h = in.res_stride_h;
     a.res_len = in.res_len; a.res_len_dev = in.res_len_dev;
     a.scale_log2 = (in.scale > 0.0f ? in.scale : 1.0f / std::sqrt(static_cast<float>(in.head_dim))) * kLog2e;
-    const Split sp = splits(in.n_prob, in.head_dim, in.n_sel < 0 ? in.n_rows : in.n_sel, in.res_len + (in.k_new ? 1 : 0));
+    const Split sp = splits(in.n_prob, in.head_dim, in.n_sel >= 0, in.n_sel < 0 ? in.n_rows : in.n_sel, in.res_len + (in.k_new ? 1 : 0));
     a.n_store_split = sp.store;
     a.n_split = sp.total;
     a.part_acc = static_cast<float*>(in.scratch);
