@@ -12,6 +12,7 @@ LIB_PATH = os.path.join(LIB_DIR, "libdiffcache_b200.so")
 SOURCES = ["scan.cu", "scan_tc.cu", "select.cu", "attend.cu", "pq.cu", "budget.cu", "exchange.cu",
            "quant.cu", "scan_q4.cu", "attend_q4.cu", "engine.cu"]
 HEADERS = [os.path.join(CSRC, "common.cuh"), os.path.join(CSRC, "exchange.cuh"), os.path.join(CSRC, "q4.cuh"),
+           os.path.join(CSRC, "q4_mma.cuh"),
            os.path.join(_HERE, "..", "include", "diffcache_b200.h")]
 
 NVCC_FLAGS = [

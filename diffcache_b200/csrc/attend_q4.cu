@@ -5,7 +5,7 @@
 #include <cmath>
 
 #include "exchange.cuh"
-#include "q4.cuh"
+#include "q4_mma.cuh"
 
 namespace dc {
 
@@ -48,29 +48,6 @@ struct Args {
     float* part_acc;                 // (n_prob, group, n_split, D)
     float* part_ml;                  // (n_prob, group, n_split, 2)
 };
-
-template <bool BF16>
-__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    if (BF16)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-// The first product of a sum: nothing to add to.
-template <bool BF16>
-__device__ __forceinline__ void mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    if (BF16)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
-                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
-    else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
-                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
-}
 
 // ---- a tile of 16 store rows in shared memory, private to one warp ----
 // Asynchronous copies of 16 (codes) and 4 / 8 / 16 bytes (a row's scales); with `ok` false zeros are written instead.
@@ -121,47 +98,6 @@ constexpr size_t attend_smem_bytes() {
     return ring > merge ? ring : merge;
 }
 
-// Constants of the code conversion, kept in registers: with an immediate operand the packed 16-bit subtraction issues to
-// the integer pipe, which the masks already fill, instead of the FMA pipe.
-struct CodeConst {
-    uint32_t f16_one, f16_off, f16_16th, f16_off16, bf16_one, bf16_off;
-    __device__ __forceinline__ explicit CodeConst(uint32_t zero) {   // 0, in a form the compiler cannot fold
-        f16_one = 0x64006400u | zero;    // 1024, 1024
-        f16_off = 0xE408E408u | zero;    // -1032
-        f16_16th = 0x2C002C00u | zero;   // 1 / 16
-        f16_off16 = 0xD480D480u | zero;  // -72
-        bf16_one = 0x43004300u | zero;   // 128, 128
-        bf16_off = 0xC308C308u | zero;   // -136
-    }
-};
-
-// Four pairs of codes of a word: pair j = (nibble j, nibble j + 4).  Inserting a nibble into the mantissa of 1024 (fp16) or
-// 128 (bf16) makes it that number plus the nibble, exactly; the offset and the 8 of the encoding go with one operation.
-__device__ __forceinline__ void codes_f16(const CodeConst& k, uint32_t w, uint32_t (&p)[4]) {
-    const uint32_t hi = w >> 8;
-    const uint32_t t[4] = {(w & 0x000F000Fu) | k.f16_one, (w & 0x00F000F0u) | k.f16_one, (hi & 0x000F000Fu) | k.f16_one,
-                           (hi & 0x00F000F0u) | k.f16_one};
-    asm("add.f16x2 %0, %1, %2;\n" : "=r"(p[0]) : "r"(t[0]), "r"(k.f16_off));
-    asm("fma.rn.f16x2 %0, %1, %2, %3;\n" : "=r"(p[1]) : "r"(t[1]), "r"(k.f16_16th), "r"(k.f16_off16));
-    asm("add.f16x2 %0, %1, %2;\n" : "=r"(p[2]) : "r"(t[2]), "r"(k.f16_off));
-    asm("fma.rn.f16x2 %0, %1, %2, %3;\n" : "=r"(p[3]) : "r"(t[3]), "r"(k.f16_16th), "r"(k.f16_off16));
-}
-__device__ __forceinline__ void codes_bf16(const CodeConst& k, uint32_t w, uint32_t (&p)[4]) {
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const uint32_t t = ((w >> (4 * i)) & 0x000F000Fu) | k.bf16_one;
-        asm("add.bf16x2 %0, %1, %2;\n" : "=r"(p[i]) : "r"(t), "r"(k.bf16_off));
-    }
-}
-
-// (x, y) rounded to a pair of 16-bit values, x in the low half; what is lost goes to a second pair.
-template <bool BF16>
-__device__ __forceinline__ uint32_t pack2(float x, float y) {
-    uint32_t r;
-    if (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(y), "f"(x));
-    else asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(y), "f"(x));
-    return r;
-}
 // The pair of weights (x, y) as B operand of a head's two column groups: hi = rounded to 16 bits, rest = rounded remainder.
 // With few heads (FEW) the lanes of rows g < 4 need hi, the others rest: `keep_lo` / `keep_hi` are byte selectors that read
 // the rounded halves as floats there, and zeros in the lanes g < 4, so that one expression serves both.
@@ -178,13 +114,6 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t keep_lo, u
         hi = FEW && keep_lo != 0x4444u ? rest : r;
     }
 }
-template <int DT>
-__device__ __forceinline__ float low_elem(uint32_t w) { return elem_to_float<DT>(static_cast<uint16_t>(w & 0xFFFFu)); }
-template <int DT>
-__device__ __forceinline__ float high_elem(uint32_t w) {
-    return DT == DC_BF16 ? __uint_as_float(w & 0xFFFF0000u) : elem_to_float<DT>(static_cast<uint16_t>(w >> 16));
-}
-
 __device__ __forceinline__ float exp2_fast(float x) {   // 2^x to 2 ulp, 0 below 2^-126 and for -inf
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(x));
@@ -309,10 +238,9 @@ q4_attend_kernel(const Args a) {
         for (int d = t; d < D; d += 4) top = fmaxf(top, fabsf(elem_to_float<DT>(qrow[d])));
         top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-        int ex = static_cast<int>((__float_as_uint(top) >> 23) & 255u);   // 0: zero or subnormal, 255: infinite
-        ex = ex == 255 ? 127 + 14 : max(ex, 28);
-        const float down = __uint_as_float(static_cast<uint32_t>(127 + 14 - ex + 127) << 23);   // 2^(14 - e)
-        const float up_g = __uint_as_float(static_cast<uint32_t>(ex - 14) << 23) * a.scale_log2;  // 2^(e - 14)
+        float down, up_g;
+        q4_normalise(top, down, up_g);
+        up_g *= a.scale_log2;
         const float up[2] = {__shfl_sync(0xFFFFFFFFu, up_g, 8 * t), __shfl_sync(0xFFFFFFFFu, up_g, 8 * t + 4)};   // heads 2t, 2t + 1
         uint32_t qa[NT][2];
 #pragma unroll
