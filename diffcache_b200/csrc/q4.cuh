@@ -37,81 +37,108 @@ inline int64_t q4_scale_bytes(int head_dim) { return head_dim / kQ4Group * 2; }
 template <int DT>
 __device__ __forceinline__ float q4_scale_max() { return DT == DC_BF16 ? 145.0f * 332306998946228968225951765070086144.0f : 9352.0f; }
 
-// Position of 8-element vector v of a row among its 32-bit code words: v = 2 * tile + half, tile = 4w + x; after
-// the exchange in q4_transpose the thread owns word w of chunk 4 * half + x.
+// A thread works on one tile (16 elements, 32 bytes) of a row: tile v of head_dim / 16, the threads of a row being
+// consecutive lanes.  Four threads (v = 4w + x) exchange bytes so that thread x ends up with word w of chunks x and 4 + x
+// (q4_word_index of both), i.e. a row leaves as full 32-byte runs.
 template <int D>
-__device__ __forceinline__ int q4_word_index(int v) {
-    const int half = v & 1, x = (v >> 1) & 3, w = v >> 3;
-    return (4 * half + x) * (D / 64) + w;
-}
+__device__ __forceinline__ int q4_word_index(int v, int half) { return (4 * half + (v & 3)) * (D / 64) + (v >> 2); }
 
-// Four threads (x = bits 1, 2 of v) hold one tile each, byte k of `word` = the pair that belongs to chunk 4h + k;
-// afterwards thread x holds chunk 4h + x of the four tiles, in the stored byte order.  Two exchanges.
+// Byte k of `word` = the pair of this thread's tile that belongs to chunk 4 * half + k; afterwards thread x holds chunk
+// 4 * half + x of the four tiles, in the stored byte order.  Two exchanges.  All lanes of a warp take part.
 __device__ __forceinline__ uint32_t q4_transpose_out(uint32_t word, int v) {
-    uint32_t r = __shfl_xor_sync(0xFFFFFFFFu, word, 2);
-    word = __byte_perm(word, r, (v & 2) ? 0x3715 : 0x6240);
-    r = __shfl_xor_sync(0xFFFFFFFFu, word, 4);
-    return __byte_perm(word, r, (v & 4) ? 0x3726 : 0x5140);
+    uint32_t r = __shfl_xor_sync(0xFFFFFFFFu, word, 1);
+    word = __byte_perm(word, r, (v & 1) ? 0x3715 : 0x6240);
+    r = __shfl_xor_sync(0xFFFFFFFFu, word, 2);
+    return __byte_perm(word, r, (v & 2) ? 0x3726 : 0x5140);
 }
 __device__ __forceinline__ uint32_t q4_transpose_in(uint32_t word, int v) {
     word = __byte_perm(word, 0u, 0x3120);
-    uint32_t r = __shfl_xor_sync(0xFFFFFFFFu, word, 4);
-    word = __byte_perm(word, r, (v & 4) ? 0x3276 : 0x5410);
-    r = __shfl_xor_sync(0xFFFFFFFFu, word, 2);
-    return __byte_perm(word, r, (v & 2) ? 0x3715 : 0x6240);
+    uint32_t r = __shfl_xor_sync(0xFFFFFFFFu, word, 2);
+    word = __byte_perm(word, r, (v & 2) ? 0x3276 : 0x5410);
+    r = __shfl_xor_sync(0xFFFFFFFFu, word, 1);
+    return __byte_perm(word, r, (v & 1) ? 0x3715 : 0x6240);
 }
 
-// Eight elements (vector v of a row) -> the code word this thread stores (at q4_word_index) and its group's scale.
-// All 32 lanes of a warp must take part; the head_dim / 8 lanes of a row are consecutive.
+// The scale of a group from its largest magnitude bits (of the element type); `inv` is about 1 / scale, 0 where the codes
+// are all zero.  max|x| / 7 is never nearer than 2^-15 (relative) to a midpoint between two numbers of the type, so one
+// fp32 product rounds to the same scale as the exact quotient.
+template <int DT>
+__device__ __forceinline__ uint16_t q4_scale(uint32_t top_bits, float& inv) {
+    inv = 0.0f;
+    if (top_bits >= (DT == DC_BF16 ? 0x7F80u : 0x7C00u)) return 0x7FFF;   // a NaN or an infinity in the group
+    const float top = elem_to_float<DT>(static_cast<uint16_t>(top_bits));
+    const uint16_t sb = float_to_elem<DT>(fminf(top * (1.0f / 7.0f), q4_scale_max<DT>()));
+    const float s = elem_to_float<DT>(sb);
+    if (s < 1.17549435e-38f) return 0;
+    asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(inv) : "f"(s));
+    return sb;
+}
+
+// Eight elements -> their eight nibbles (c + 8), element i in bits 4i.
 //
 // The quotient is rounded exactly as defined without a division per element: x / s is either exactly a half-integer
-// or at least 2^-12 away from one (x and s have at most 11 significant bits), x * (1 / s) is off by less than 2^-20,
-// and fma(x, 1 / s, 1536) rounds to a multiple of 2^-13: a tie lands exactly on the half-integer, nothing else does.
+// or at least 2^-12 away from one (x and s have at most 11 significant bits), x * inv is off by less than 2^-19,
+// and fma(x, inv, 1536) rounds to a multiple of 2^-13: a tie lands exactly on the half-integer, nothing else does.
 // The second addition then rounds half to even (1.5 * 2^23 + 8 is even), leaving c + 8 in the low bits.
 template <int DT>
-__device__ __forceinline__ uint32_t q4_encode8(const uint4& w, int v, uint16_t& scale) {
-    const uint32_t kAbs = 0x7FFF7FFFu;
-    uint32_t m = __vmaxu2(__vmaxu2(w.x & kAbs, w.y & kAbs), __vmaxu2(w.z & kAbs, w.w & kAbs));
-    m = max(m & 0xFFFFu, m >> 16);
-    m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
-    m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));   // magnitude bits order like magnitudes; NaN and inf on top
-    const bool finite = m < (DT == DC_BF16 ? 0x7F80u : 0x7C00u);
-    const float top = finite ? elem_to_float<DT>(static_cast<uint16_t>(m)) : 0.0f;
-    uint16_t sb = float_to_elem<DT>(fminf(__fdiv_rn(top, 7.0f), q4_scale_max<DT>()));
-    float s = elem_to_float<DT>(sb);
-    if (s < 1.17549435e-38f) { s = 0.0f; sb = 0; }
-    const float inv = s > 0.0f ? __frcp_rn(s) : 0.0f;
-    scale = finite ? sb : static_cast<uint16_t>(0x7FFF);
+__device__ __forceinline__ uint32_t q4_codes8(const uint4& w, float inv) {
     float f[8];
     unpack8<DT>(w, f);
-    uint32_t word = 0;
+    uint32_t word = 0, bias = 0;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        // a group of magnitude 0 or one that is not finite has code 0 throughout (0 * inf never forms)
-        float t = finite ? fmaf(f[i], inv, 1536.0f) : 1536.0f;
+        float t = fmaf(f[i], inv, 1536.0f);
         if (DT == DC_FP16) t = fminf(fmaxf(t, 1529.0f), 1543.0f);   // a subnormal scale can be off by up to a half
         word += __float_as_uint(t + (12582920.0f - 1536.0f)) << (4 * i);
+        bias += 0x4B400000u << (4 * i);                             // the bits of 1.5 * 2^23, in every term
     }
-    // every term carries the bits of 1.5 * 2^23 as well: their sum over i is a constant
-    uint32_t bias = 0;
-#pragma unroll
-    for (int i = 0; i < 8; i++) bias += 0x4B400000u << (4 * i);
-    return q4_transpose_out(word - bias, v);
+    return word - bias;
 }
 
-// The inverse: the code word stored at q4_word_index and the group's scale -> eight elements, s * c rounded once.
+// One tile -> the two code words this thread stores (chunks x and 4 + x) and its group's scale.  All lanes take part.
 template <int DT>
-__device__ __forceinline__ uint4 q4_decode8(uint32_t word, uint16_t scale, int v) {
-    word = q4_transpose_in(word, v);
-    const float s = elem_to_float<DT>(scale);
-    uint32_t o[4];
+__device__ __forceinline__ void q4_encode(const uint4 (&w)[2], int v, uint32_t (&word)[2], uint16_t& scale) {
+    const uint32_t kAbs = 0x7FFF7FFFu;
+    uint32_t m = __vmaxu2(__vmaxu2(__vmaxu2(w[0].x & kAbs, w[0].y & kAbs), __vmaxu2(w[0].z & kAbs, w[0].w & kAbs)),
+                          __vmaxu2(__vmaxu2(w[1].x & kAbs, w[1].y & kAbs), __vmaxu2(w[1].z & kAbs, w[1].w & kAbs)));
+    m = __vmaxu2(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));   // magnitude bits order like magnitudes; NaN and inf on top
+    m = max(m & 0xFFFFu, m >> 16);
+    float inv;
+    scale = q4_scale<DT>(m, inv);
+    // a group whose codes are all zero must not multiply (0 * inf): its elements are replaced by zeros
+    const bool live = inv != 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float a = __uint_as_float(0x4B000000u | ((word >> (8 * i)) & 15u)) - 8388616.0f;
-        const float b = __uint_as_float(0x4B000000u | ((word >> (8 * i + 4)) & 15u)) - 8388616.0f;
-        o[i] = float_to_elem<DT>(a * s) | (static_cast<uint32_t>(float_to_elem<DT>(b * s)) << 16);
+    for (int h = 0; h < 2; h++) {
+        const uint32_t c = q4_codes8<DT>(w[h], inv);
+        word[h] = q4_transpose_out(live ? c : 0x88888888u, v);
     }
-    return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+// The inverse: the two code words and the group's scale -> the tile, s * c rounded once (a packed 16-bit product of exact
+// operands rounds the exact result).
+template <int DT>
+__device__ __forceinline__ void q4_decode(const uint32_t (&word)[2], uint16_t scale, int v, uint4 (&out)[2]) {
+    const uint32_t s2 = scale * 0x10001u;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const uint32_t w = q4_transpose_in(word[h], v);   // byte k: elements (2k, 2k + 1) of this half tile
+        const uint32_t lo = w & 0x0F0F0F0Fu, hi = (w >> 4) & 0x0F0F0F0Fu;
+        uint32_t o[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const uint32_t pair = __byte_perm(lo, hi, k * 0x0011 + (4 + k) * 0x1100) & 0x000F000Fu;
+            if (DT == DC_BF16) {
+                uint32_t c;
+                asm("sub.bf16x2 %0, %1, %2;\n" : "=r"(c) : "r"(pair | 0x43004300u), "r"(0x43084308u));
+                asm("mul.rn.bf16x2 %0, %1, %2;\n" : "=r"(o[k]) : "r"(c), "r"(s2));
+            } else {
+                uint32_t c;
+                asm("sub.f16x2 %0, %1, %2;\n" : "=r"(c) : "r"(pair | 0x64006400u), "r"(0x64086408u));
+                asm("mul.rn.f16x2 %0, %1, %2;\n" : "=r"(o[k]) : "r"(c), "r"(s2));
+            }
+        }
+        out[h] = make_uint4(o[0], o[1], o[2], o[3]);
+    }
 }
 
 // ---- host side (quant.cu, scan_q4.cu, attend_q4.cu) ----

@@ -4,15 +4,16 @@
 // (diffcache_cpu/src/lib.rs:329-369, nsw.rs:497-557) and the row gather of search_bruteforce (nsw.rs:621-629),
 // which the reference does with plain copies.
 //
-// A thread holds 8 consecutive elements (one 16-byte load); the group maximum is two shuffles, the codes move to
-// their stored order with two more, and the row leaves as 4-byte words that the head_dim / 8 threads of a row write
-// side by side.  Bound: HBM (2 * head_dim bytes in, 9/16 * head_dim out per row, or the other way round).
+// A thread holds one tile, 16 consecutive elements (32 bytes): the group maximum is one shuffle away, the codes move to their
+// stored order with four more, and a row leaves as runs of 32 bytes.  Several rows per thread are loaded before the first is
+// worked on.  Bound: HBM (2 * head_dim bytes in, 9/16 * head_dim out per row, or the other way round).
 #include "q4.cuh"
 
 namespace dc {
 namespace {
 
 constexpr int kRowThreads = 256;
+constexpr int kRowsPerThread = 4;
 
 struct WriteArgs {
     const uint16_t* src[2];     // keys, values
@@ -24,10 +25,17 @@ struct WriteArgs {
     int len_mode;
 };
 
+__device__ __forceinline__ void load_tile(const uint16_t* p, uint4 (&w)[2]) {   // 16-byte aligned
+    w[0] = ld_stream16(p);
+    w[1] = ld_stream16(p + 8);
+}
+
 template <int D>
-__device__ __forceinline__ void q4_put(const Q4Rows& t, int64_t row, int v, uint32_t word, uint16_t scale) {
-    reinterpret_cast<uint32_t*>(t.codes + row * (D / 2))[q4_word_index<D>(v)] = word;
-    if ((v & 3) == 0) t.scales[row * (D / kQ4Group) + (v >> 2)] = scale;
+__device__ __forceinline__ void q4_put(const Q4Rows& t, int64_t row, int v, const uint32_t (&word)[2], uint16_t scale) {
+    uint32_t* c = reinterpret_cast<uint32_t*>(t.codes + row * (D / 2));
+    c[q4_word_index<D>(v, 0)] = word[0];
+    c[q4_word_index<D>(v, 1)] = word[1];
+    if ((v & 1) == 0) t.scales[row * (D / kQ4Group) + (v >> 1)] = scale;
 }
 
 // grid = (row blocks, n_prob, 2 tensors)
@@ -36,17 +44,28 @@ __global__ void __launch_bounds__(kRowThreads)
 q4_write_kernel(const WriteArgs a) {
     pdl_launch_dependents();
     pdl_wait();
-    constexpr int LPR = D / 8, RPB = kRowThreads / LPR;
+    constexpr int LPR = D / 16, RPB = kRowThreads / LPR;
     const int64_t prob = blockIdx.y;
     const int v = threadIdx.x % LPR;
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * RPB + threadIdx.x / LPR;
-    const bool ok = i < a.n;
+    const int64_t i0 = static_cast<int64_t>(blockIdx.x) * (RPB * kRowsPerThread) + threadIdx.x / LPR;
     const int64_t b = prob / a.kv_heads, h = prob % a.kv_heads;
-    uint4 w = make_uint4(0, 0, 0, 0);
-    if (ok) w = ld_stream16(a.src[blockIdx.z] + b * a.stride_b + h * a.stride_h + i * a.stride_s + v * 8);
-    uint16_t scale;
-    const uint32_t word = q4_encode8<DT>(w, v, scale);
-    if (ok) q4_put<D>(blockIdx.z ? a.st.v : a.st.k, prob * a.st.prob_rows + a.row0 + i, v, word, scale);
+    const uint16_t* src = a.src[blockIdx.z] + b * a.stride_b + h * a.stride_h + v * 16;
+    uint4 w[kRowsPerThread][2];
+#pragma unroll
+    for (int r = 0; r < kRowsPerThread; r++) {
+        const int64_t i = i0 + r * RPB;
+        w[r][0] = w[r][1] = make_uint4(0, 0, 0, 0);
+        if (i < a.n) load_tile(src + i * a.stride_s, w[r]);
+    }
+    const Q4Rows& dst = blockIdx.z ? a.st.v : a.st.k;
+#pragma unroll
+    for (int r = 0; r < kRowsPerThread; r++) {
+        const int64_t i = i0 + r * RPB;
+        uint32_t word[2];
+        uint16_t scale;
+        q4_encode<DT>(w[r], v, word, scale);
+        if (i < a.n) q4_put<D>(dst, prob * a.st.prob_rows + a.row0 + i, v, word, scale);
+    }
     if (a.len_mode != kLenKeep && blockIdx.x == 0 && prob == 0 && blockIdx.z == 0 && threadIdx.x == 0) {
         const int32_t end = static_cast<int32_t>(a.row0 + a.n);
         a.len[0] = a.len_mode == kLenSet ? end : max(a.len[0], end);
@@ -59,7 +78,7 @@ template <int DT, int D>
 __global__ void __launch_bounds__(1024)
 q4_append_kernel(const uint16_t* __restrict__ keys, const uint16_t* __restrict__ vals, int n_prob, const Q4Store st,
                  int64_t max_rows, int32_t* len, uint32_t* status) {
-    constexpr int LPR = D / 8;
+    constexpr int LPR = D / 16;
     const int64_t n = len[0];
     if (n >= max_rows) {   // full: nothing is written (the host-side call reports it when it can tell)
         if (threadIdx.x == 0 && status) atomicMax(status, 301u);
@@ -70,10 +89,11 @@ q4_append_kernel(const uint16_t* __restrict__ keys, const uint16_t* __restrict__
         const int i = i0 + threadIdx.x;
         const bool ok = i < total;
         const int p = i / (2 * LPR), which = (i / LPR) & 1, v = i % LPR;
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (ok) w = *reinterpret_cast<const uint4*>((which ? vals : keys) + static_cast<int64_t>(p) * D + v * 8);
+        uint4 w[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+        if (ok) load_tile((which ? vals : keys) + static_cast<int64_t>(p) * D + v * 16, w);
+        uint32_t word[2];
         uint16_t scale;
-        const uint32_t word = q4_encode8<DT>(w, v, scale);
+        q4_encode<DT>(w, v, word, scale);
         if (ok) q4_put<D>(which ? st.v : st.k, p * st.prob_rows + n, v, word, scale);
     }
     __syncthreads();
@@ -90,7 +110,7 @@ q4_window_push_kernel(const uint16_t* __restrict__ k_new, const uint16_t* __rest
                       int32_t* win, uint32_t* status) {
     pdl_launch_dependents();
     pdl_wait();
-    constexpr int LPR = D / 8;
+    constexpr int LPR = D / 16;
     const int suffix_len = win[0], head = win[1], prefix_len = win[2], cap = win[3];
     const int64_t n = len[0];
     const bool full = suffix_len >= cap;
@@ -104,16 +124,24 @@ q4_window_push_kernel(const uint16_t* __restrict__ k_new, const uint16_t* __rest
         const int p = i / (2 * LPR), which = (i / LPR) & 1, v = i % LPR;
         const int b = p / kv_heads, h = p % kv_heads;
         uint16_t* row = (which ? res_v : res_k) + b * res_stride_b + h * res_stride_h +
-                        static_cast<int64_t>(prefix_len + slot) * D + v * 8;
+                        static_cast<int64_t>(prefix_len + slot) * D + v * 16;
         if (spill) {
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (ok) w = *reinterpret_cast<const uint4*>(row);
+            uint4 w[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+            if (ok) {
+                w[0] = reinterpret_cast<const uint4*>(row)[0];
+                w[1] = reinterpret_cast<const uint4*>(row)[1];
+            }
+            uint32_t word[2];
             uint16_t scale;
-            const uint32_t word = q4_encode8<DT>(w, v, scale);
+            q4_encode<DT>(w, v, word, scale);
             if (ok) q4_put<D>(which ? st.v : st.k, p * st.prob_rows + n, v, word, scale);
         }
         const int64_t off = new_stride_b ? b * new_stride_b + static_cast<int64_t>(h) * D : static_cast<int64_t>(p) * D;
-        if (ok) *reinterpret_cast<uint4*>(row) = *reinterpret_cast<const uint4*>((which ? v_new : k_new) + off + v * 8);
+        if (ok) {
+            const uint4* fresh = reinterpret_cast<const uint4*>((which ? v_new : k_new) + off + v * 16);
+            reinterpret_cast<uint4*>(row)[0] = fresh[0];
+            reinterpret_cast<uint4*>(row)[1] = fresh[1];
+        }
     }
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -137,33 +165,54 @@ __global__ void __launch_bounds__(kRowThreads)
 q4_read_kernel(const ReadArgs a) {
     pdl_launch_dependents();
     pdl_wait();
-    constexpr int LPR = D / 8, RPB = kRowThreads / LPR;
+    constexpr int LPR = D / 16, RPB = kRowThreads / LPR;
     const int64_t prob = blockIdx.y;
     const int v = threadIdx.x % LPR;
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * RPB + threadIdx.x / LPR;
+    const int64_t i0 = static_cast<int64_t>(blockIdx.x) * (RPB * kRowsPerThread) + threadIdx.x / LPR;
     const int which = a.out[0] == nullptr ? 1 : blockIdx.z;
     const int64_t n_rows = a.n_dev != nullptr ? static_cast<int64_t>(*a.n_dev) : a.n_rows;
-    uint32_t word = 0x88888888u;
-    uint16_t scale = 0;
-    if (i < a.n) {
-        const int64_t row = a.ids != nullptr ? static_cast<int64_t>(a.ids[prob * a.ids_stride + i]) : a.row0 + i;
-        if (row < n_rows) {   // a pad (0xFFFFFFFF) or any id beyond the stored rows reads as zeros
-            const Q4Rows& t = which ? a.st.v : a.st.k;
-            const int64_t r = prob * a.st.prob_rows + row;
-            word = __ldcs(reinterpret_cast<const uint32_t*>(t.codes + r * (D / 2)) + q4_word_index<D>(v));
-            scale = t.scales[r * (D / kQ4Group) + (v >> 2)];
+    const Q4Rows& t = which ? a.st.v : a.st.k;
+    uint32_t word[kRowsPerThread][2];
+    uint16_t scale[kRowsPerThread];
+#pragma unroll
+    for (int r = 0; r < kRowsPerThread; r++) {
+        const int64_t i = i0 + r * RPB;
+        word[r][0] = word[r][1] = 0x88888888u;
+        scale[r] = 0;
+        if (i < a.n) {
+            const int64_t row = a.ids != nullptr ? static_cast<int64_t>(a.ids[prob * a.ids_stride + i]) : a.row0 + i;
+            if (row < n_rows) {   // a pad (0xFFFFFFFF) or any id beyond the stored rows reads as zeros
+                const int64_t at = prob * a.st.prob_rows + row;
+                const uint32_t* c = reinterpret_cast<const uint32_t*>(t.codes + at * (D / 2));
+                word[r][0] = __ldcs(c + q4_word_index<D>(v, 0));
+                word[r][1] = __ldcs(c + q4_word_index<D>(v, 1));
+                scale[r] = t.scales[at * (D / kQ4Group) + (v >> 1)];
+            }
         }
     }
-    if (F32) {
-        word = q4_transpose_in(word, v);
-        if (i >= a.n) return;
-        const float s = elem_to_float<DT>(scale);
-        float* o = static_cast<float*>(a.out[which]) + (prob * a.n + i) * D + v * 8;
 #pragma unroll
-        for (int e = 0; e < 8; e++) o[e] = static_cast<float>(static_cast<int>((word >> (4 * e)) & 15u) - 8) * s;
-    } else {
-        const uint4 w = q4_decode8<DT>(word, scale, v);
-        if (i < a.n) __stcs(reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out[which]) + (prob * a.n + i) * D + v * 8), w);
+    for (int r = 0; r < kRowsPerThread; r++) {
+        const int64_t i = i0 + r * RPB;
+        const int64_t at = (prob * a.n + i) * D + v * 16;
+        if (F32) {
+            const float s = elem_to_float<DT>(scale[r]);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const uint32_t w = q4_transpose_in(word[r][h], v);
+                if (i < a.n)
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        static_cast<float*>(a.out[which])[at + 8 * h + e] = static_cast<float>(static_cast<int>((w >> (4 * e)) & 15u) - 8) * s;
+            }
+        } else {
+            uint4 o[2];
+            q4_decode<DT>(word[r], scale[r], v, o);
+            if (i < a.n) {
+                uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out[which]) + at);
+                __stcs(dst, o[0]);
+                __stcs(dst + 1, o[1]);
+            }
+        }
     }
 }
 
@@ -192,7 +241,7 @@ int q4_write_rows(const void* keys, const void* vals, int64_t stride_b, int64_t 
     a.n = n; a.row0 = row0;
     a.st = st;
     a.len = len; a.len_mode = len_mode;
-    const int64_t rpb = kRowThreads / (head_dim / 8);
+    const int64_t rpb = kRowThreads / (head_dim / 16) * kRowsPerThread;
     const dim3 grid(static_cast<unsigned>(n > 0 ? (n + rpb - 1) / rpb : 1), static_cast<unsigned>(n_prob), 2u);
 #define CASE(DT, D) DC_CUDA_TRY(launch_chained(q4_write_kernel<DT, D>, grid, dim3(kRowThreads), 0, stream, 0u, a))
     DC_Q4_DISPATCH(dtype, head_dim, CASE)
@@ -233,7 +282,7 @@ int q4_read_rows(const Q4Store& st, int64_t n_rows, const int32_t* n_dev, int n_
     a.ids = ids; a.ids_stride = ids_stride;
     a.row0 = row0; a.n = n;
     a.out[0] = out_k; a.out[1] = out_v;
-    const int64_t rpb = kRowThreads / (head_dim / 8);
+    const int64_t rpb = kRowThreads / (head_dim / 16) * kRowsPerThread;
     const dim3 grid(static_cast<unsigned>((n + rpb - 1) / rpb), static_cast<unsigned>(n_prob), out_k && out_v ? 2u : 1u);
 #define CASE(DT, D)                                                                                             \
     if (f32) DC_CUDA_TRY(launch_chained(q4_read_kernel<DT, D, true>, grid, dim3(kRowThreads), 0, stream, 0u, a)); \
