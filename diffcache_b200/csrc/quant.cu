@@ -5,18 +5,21 @@
 // which the reference does with plain copies.
 //
 // A thread holds one tile, 16 consecutive elements (32 bytes): the group maximum is one shuffle away, the codes move to their
-// stored order with four more, and a row leaves as runs of 32 bytes.  Several rows per thread are loaded before the first is
-// worked on.  Bound: HBM (2 * head_dim bytes in, 9/16 * head_dim out per row, or the other way round).
+// stored order with four more, and a row leaves as runs of 32 bytes.  Bound: HBM (2 * head_dim bytes in, 9/16 * head_dim out per row, or the other way round).
 #include "q4.cuh"
 
 namespace dc {
 namespace {
 
 constexpr int kRowThreads = 256;
-constexpr int kRowsPerThread = 4;
+// Rows a thread of the write kernel loads before it works on the first.  4 x 8 x 130496 rows of head_dim 128, keys and values:
+// 522 us with one, 445 with two (6.16 TB/s), 443 with four; a single token 2.5, 2.8, 3.3 us.  Reading back does best with
+// one row per thread (448 us, 6.12 TB/s; 452 with two, 524 with four).
+constexpr int kWriteRows = 2;
 
 struct WriteArgs {
-    const uint16_t* src[2];     // keys, values
+    const uint16_t* keys;
+    const uint16_t* vals;
     int64_t stride_b, stride_h, stride_s;
     int kv_heads;
     int64_t n, row0;
@@ -24,6 +27,11 @@ struct WriteArgs {
     int32_t* len;
     int len_mode;
 };
+
+// (field by field: a reference into the kernel's parameters would copy them to local memory)
+__device__ __forceinline__ Q4Rows pick(const Q4Store& st, int values) {
+    return {values ? st.v.codes : st.k.codes, values ? st.v.scales : st.k.scales};
+}
 
 __device__ __forceinline__ void load_tile(const uint16_t* p, uint4 (&w)[2]) {   // 16-byte aligned
     w[0] = ld_stream16(p);
@@ -47,19 +55,19 @@ q4_write_kernel(const WriteArgs a) {
     constexpr int LPR = D / 16, RPB = kRowThreads / LPR;
     const int64_t prob = blockIdx.y;
     const int v = threadIdx.x % LPR;
-    const int64_t i0 = static_cast<int64_t>(blockIdx.x) * (RPB * kRowsPerThread) + threadIdx.x / LPR;
+    const int64_t i0 = static_cast<int64_t>(blockIdx.x) * (RPB * kWriteRows) + threadIdx.x / LPR;
     const int64_t b = prob / a.kv_heads, h = prob % a.kv_heads;
-    const uint16_t* src = a.src[blockIdx.z] + b * a.stride_b + h * a.stride_h + v * 16;
-    uint4 w[kRowsPerThread][2];
+    const uint16_t* src = (blockIdx.z ? a.vals : a.keys) + b * a.stride_b + h * a.stride_h + v * 16;
+    uint4 w[kWriteRows][2];
 #pragma unroll
-    for (int r = 0; r < kRowsPerThread; r++) {
+    for (int r = 0; r < kWriteRows; r++) {
         const int64_t i = i0 + r * RPB;
         w[r][0] = w[r][1] = make_uint4(0, 0, 0, 0);
         if (i < a.n) load_tile(src + i * a.stride_s, w[r]);
     }
-    const Q4Rows& dst = blockIdx.z ? a.st.v : a.st.k;
+    const Q4Rows dst = pick(a.st, blockIdx.z);
 #pragma unroll
-    for (int r = 0; r < kRowsPerThread; r++) {
+    for (int r = 0; r < kWriteRows; r++) {
         const int64_t i = i0 + r * RPB;
         uint32_t word[2];
         uint16_t scale;
@@ -94,7 +102,7 @@ q4_append_kernel(const uint16_t* __restrict__ keys, const uint16_t* __restrict__
         uint32_t word[2];
         uint16_t scale;
         q4_encode<DT>(w, v, word, scale);
-        if (ok) q4_put<D>(which ? st.v : st.k, p * st.prob_rows + n, v, word, scale);
+        if (ok) q4_put<D>(pick(st, which), p * st.prob_rows + n, v, word, scale);
     }
     __syncthreads();
     if (threadIdx.x == 0) len[0] = static_cast<int32_t>(n + 1);
@@ -134,7 +142,7 @@ q4_window_push_kernel(const uint16_t* __restrict__ k_new, const uint16_t* __rest
             uint32_t word[2];
             uint16_t scale;
             q4_encode<DT>(w, v, word, scale);
-            if (ok) q4_put<D>(which ? st.v : st.k, p * st.prob_rows + n, v, word, scale);
+            if (ok) q4_put<D>(pick(st, which), p * st.prob_rows + n, v, word, scale);
         }
         const int64_t off = new_stride_b ? b * new_stride_b + static_cast<int64_t>(h) * D : static_cast<int64_t>(p) * D;
         if (ok) {
@@ -156,7 +164,8 @@ struct ReadArgs {
     const int32_t* n_dev;
     const uint32_t* ids;        // (n_prob, ids_stride) or NULL: rows row0, row0 + 1, ...
     int64_t ids_stride, row0, n;
-    void* out[2];
+    void* out_k;                // either may be NULL
+    void* out_v;
 };
 
 // grid = (row blocks, n_prob, outputs)
@@ -168,50 +177,41 @@ q4_read_kernel(const ReadArgs a) {
     constexpr int LPR = D / 16, RPB = kRowThreads / LPR;
     const int64_t prob = blockIdx.y;
     const int v = threadIdx.x % LPR;
-    const int64_t i0 = static_cast<int64_t>(blockIdx.x) * (RPB * kRowsPerThread) + threadIdx.x / LPR;
-    const int which = a.out[0] == nullptr ? 1 : blockIdx.z;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * RPB + threadIdx.x / LPR;
+    const int which = a.out_k == nullptr ? 1 : blockIdx.z;
+    void* out = which ? a.out_v : a.out_k;
     const int64_t n_rows = a.n_dev != nullptr ? static_cast<int64_t>(*a.n_dev) : a.n_rows;
-    const Q4Rows& t = which ? a.st.v : a.st.k;
-    uint32_t word[kRowsPerThread][2];
-    uint16_t scale[kRowsPerThread];
-#pragma unroll
-    for (int r = 0; r < kRowsPerThread; r++) {
-        const int64_t i = i0 + r * RPB;
-        word[r][0] = word[r][1] = 0x88888888u;
-        scale[r] = 0;
-        if (i < a.n) {
-            const int64_t row = a.ids != nullptr ? static_cast<int64_t>(a.ids[prob * a.ids_stride + i]) : a.row0 + i;
-            if (row < n_rows) {   // a pad (0xFFFFFFFF) or any id beyond the stored rows reads as zeros
-                const int64_t at = prob * a.st.prob_rows + row;
-                const uint32_t* c = reinterpret_cast<const uint32_t*>(t.codes + at * (D / 2));
-                word[r][0] = __ldcs(c + q4_word_index<D>(v, 0));
-                word[r][1] = __ldcs(c + q4_word_index<D>(v, 1));
-                scale[r] = t.scales[at * (D / kQ4Group) + (v >> 1)];
-            }
+    const Q4Rows t = pick(a.st, which);
+    uint32_t word[2] = {0x88888888u, 0x88888888u};
+    uint16_t scale = 0;
+    if (i < a.n) {
+        const int64_t row = a.ids != nullptr ? static_cast<int64_t>(a.ids[prob * a.ids_stride + i]) : a.row0 + i;
+        if (row < n_rows) {   // a pad (0xFFFFFFFF) or any id beyond the stored rows reads as zeros
+            const int64_t at = prob * a.st.prob_rows + row;
+            const uint32_t* c = reinterpret_cast<const uint32_t*>(t.codes + at * (D / 2));
+            word[0] = __ldcs(c + q4_word_index<D>(v, 0));
+            word[1] = __ldcs(c + q4_word_index<D>(v, 1));
+            scale = t.scales[at * (D / kQ4Group) + (v >> 1)];
         }
     }
+    const int64_t at = (prob * a.n + i) * D + v * 16;
+    if (F32) {
+        const float s = elem_to_float<DT>(scale);
 #pragma unroll
-    for (int r = 0; r < kRowsPerThread; r++) {
-        const int64_t i = i0 + r * RPB;
-        const int64_t at = (prob * a.n + i) * D + v * 16;
-        if (F32) {
-            const float s = elem_to_float<DT>(scale[r]);
+        for (int h = 0; h < 2; h++) {
+            const uint32_t w = q4_transpose_in(word[h], v);
+            if (i < a.n)
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const uint32_t w = q4_transpose_in(word[r][h], v);
-                if (i < a.n)
-#pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        static_cast<float*>(a.out[which])[at + 8 * h + e] = static_cast<float>(static_cast<int>((w >> (4 * e)) & 15u) - 8) * s;
-            }
-        } else {
-            uint4 o[2];
-            q4_decode<DT>(word[r], scale[r], v, o);
-            if (i < a.n) {
-                uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out[which]) + at);
-                __stcs(dst, o[0]);
-                __stcs(dst + 1, o[1]);
-            }
+                for (int e = 0; e < 8; e++)
+                    static_cast<float*>(out)[at + 8 * h + e] = static_cast<float>(static_cast<int>((w >> (4 * e)) & 15u) - 8) * s;
+        }
+    } else {
+        uint4 o[2];
+        q4_decode<DT>(word, scale, v, o);
+        if (i < a.n) {
+            uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at);
+            __stcs(dst, o[0]);
+            __stcs(dst + 1, o[1]);
         }
     }
 }
@@ -234,14 +234,14 @@ int q4_write_rows(const void* keys, const void* vals, int64_t stride_b, int64_t 
                   int len_mode, cudaStream_t stream) {
     if (n_prob == 0 || (n == 0 && len_mode == kLenKeep)) return DC_OK;
     WriteArgs a;
-    a.src[0] = static_cast<const uint16_t*>(keys);
-    a.src[1] = static_cast<const uint16_t*>(vals);
+    a.keys = static_cast<const uint16_t*>(keys);
+    a.vals = static_cast<const uint16_t*>(vals);
     a.stride_b = stride_b; a.stride_h = stride_h; a.stride_s = stride_s;
     a.kv_heads = kv_heads;
     a.n = n; a.row0 = row0;
     a.st = st;
     a.len = len; a.len_mode = len_mode;
-    const int64_t rpb = kRowThreads / (head_dim / 16) * kRowsPerThread;
+    const int64_t rpb = kRowThreads / (head_dim / 16) * kWriteRows;
     const dim3 grid(static_cast<unsigned>(n > 0 ? (n + rpb - 1) / rpb : 1), static_cast<unsigned>(n_prob), 2u);
 #define CASE(DT, D) DC_CUDA_TRY(launch_chained(q4_write_kernel<DT, D>, grid, dim3(kRowThreads), 0, stream, 0u, a))
     DC_Q4_DISPATCH(dtype, head_dim, CASE)
@@ -281,8 +281,8 @@ int q4_read_rows(const Q4Store& st, int64_t n_rows, const int32_t* n_dev, int n_
     a.n_rows = n_rows; a.n_dev = n_dev;
     a.ids = ids; a.ids_stride = ids_stride;
     a.row0 = row0; a.n = n;
-    a.out[0] = out_k; a.out[1] = out_v;
-    const int64_t rpb = kRowThreads / (head_dim / 16) * kRowsPerThread;
+    a.out_k = out_k; a.out_v = out_v;
+    const int64_t rpb = kRowThreads / (head_dim / 16);
     const dim3 grid(static_cast<unsigned>((n + rpb - 1) / rpb), static_cast<unsigned>(n_prob), out_k && out_v ? 2u : 1u);
 #define CASE(DT, D)                                                                                             \
     if (f32) DC_CUDA_TRY(launch_chained(q4_read_kernel<DT, D, true>, grid, dim3(kRowThreads), 0, stream, 0u, a)); \
