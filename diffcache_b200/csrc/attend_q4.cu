@@ -1,6 +1,8 @@
 // Attention over a store held in 4 bits (format: q4.cuh), the resident 16-bit rows and the new token, with split-K
 // and log-sum-exp merge: the 4-bit counterpart of attend.cu (flash_attn_with_kvcache over the gathered buffer,
 // src/diffcache/base.py:134-142), over the rows of an id list or over every stored row of a sequence.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <cmath>
 
@@ -8,6 +10,8 @@
 #include "q4_mma.cuh"
 
 namespace dc {
+
+namespace cg = cooperative_groups;
 
 int lse_combine(const float* acc, int64_t acc_ps, int64_t acc_rs, const float* ml, int64_t ml_ps, int64_t ml_rs,
                 int n_part, int64_t rows, int head_dim, int dtype, void* out, float* out_lse, float* out_acc,
@@ -45,7 +49,10 @@ struct Args {
     float scale_log2;
     int n_store_split;               // CTAs (per problem and head chunk) that take store rows; the others take 16-bit rows
     int n_split;
-    float* part_acc;                 // (n_prob, group, n_split, D)
+    int in_cluster;                  // the n_split CTAs of a problem are one cluster and finish the output themselves
+    uint16_t* out;                   // then: (n_prob, group, D) and optional (n_prob, group)
+    float* out_lse;
+    float* part_acc;                 // otherwise: (n_prob, group, n_split, D)
     float* part_ml;                  // (n_prob, group, n_split, 2)
 };
 
@@ -196,6 +203,7 @@ q4_attend_kernel(const Args a) {
     extern __shared__ __align__(128) unsigned char s_ring[];   // the warps' rings; at the end their partial outputs
     __shared__ uint32_t s_ok[kWarps][Ring<D>::STAGES];         // rows of a tile that exist (id lists)
     __shared__ float s_ml[kWarps][kHeads][2];
+    __shared__ float s_sum[kHeads][2];                         // the CTA's (reference, sum), for the cluster
     {
         const uint16_t* qb = a.q_stride_b ? a.q + b * a.q_stride_b + (static_cast<int64_t>(h) * a.group + g0) * D
                                           : a.q + (prob * a.group + g0) * D;
@@ -217,7 +225,6 @@ q4_attend_kernel(const Args a) {
     float o[NT][4];
 #pragma unroll
     for (int i = 0; i < NT; i++) { o[i][0] = 0.0f; o[i][1] = 0.0f; o[i][2] = 0.0f; o[i][3] = 0.0f; }
-    __syncthreads();
 
     if (split < a.n_store_split) {
         const int64_t n_rows = a.n_rows_dev != nullptr ? min(a.n_rows, static_cast<int64_t>(*a.n_rows_dev)) : a.n_rows;
@@ -232,29 +239,6 @@ q4_attend_kernel(const Args a) {
         const uint8_t* kc = a.st.k.codes + prob * a.st.prob_rows * (D / 2);
         const uint8_t* vc = a.st.v.codes + prob * a.st.prob_rows * (D / 2);
         const uint8_t* sc_base = reinterpret_cast<const uint8_t*>((lane < 16 ? a.st.k.scales : a.st.v.scales) + prob * a.st.prob_rows * NG);
-
-        // query fragments, normalised to [2^14, 2^15) by a power of two
-        float top = 0.0f;
-        for (int d = t; d < D; d += 4) top = fmaxf(top, fabsf(elem_to_float<DT>(qrow[d])));
-        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-        float down, up_g;
-        q4_normalise(top, down, up_g);
-        up_g *= a.scale_log2;
-        const float up[2] = {__shfl_sync(0xFFFFFFFFu, up_g, 8 * t), __shfl_sync(0xFFFFFFFFu, up_g, 8 * t + 4)};   // heads 2t, 2t + 1
-        uint32_t qa[NT][2];
-#pragma unroll
-        for (int w = 0; w < D / 64; w++)
-#pragma unroll
-            for (int gp = 0; gp < 2; gp++)
-#pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    const int d = 16 * (4 * w + 2 * gp) + 2 * (2 * t + c);   // a tile's element; + 16 is the group's other tile
-#pragma unroll
-                    for (int e = 0; e < 2; e++)
-                        qa[4 * w + 2 * gp + c][e] = pack2<false>(elem_to_float<DT>(qrow[d + e]) * down,
-                                                                 elem_to_float<DT>(qrow[d + 16 + e]) * down);
-                }
 
         // ---- the ring: lane copies chunks lane + 32 j of both tensors' codes and one row's scales of one tensor ----
         using R = Ring<D>;
@@ -325,6 +309,38 @@ q4_attend_kernel(const Args a) {
 #pragma unroll
         for (int i = 0; i < 4; i++)
             v_at[i] = R::CODES + R::chunk(4 * t + i, g * (D / 16) / 16) + g * (D / 16) % 16;
+        int32_t id = IDS ? fetch_id(0) : 0;
+        if (n_mine > 0) {
+#pragma unroll
+            for (int i = 0; i < R::STAGES - 1; i++) {  // tiles beyond the last copy nothing
+                issue(ring + i * R::STAGE, i, id);
+                if (IDS) id = fetch_id(i + 1);
+            }
+        }
+        __syncthreads();                               // the query is in shared memory
+        // query fragments, normalised to [2^14, 2^15) by a power of two
+        float top = 0.0f;
+        for (int d = t; d < D; d += 4) top = fmaxf(top, fabsf(elem_to_float<DT>(qrow[d])));
+        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+        float down, up_g;
+        q4_normalise(top, down, up_g);
+        up_g *= a.scale_log2;
+        const float up[2] = {__shfl_sync(0xFFFFFFFFu, up_g, 8 * t), __shfl_sync(0xFFFFFFFFu, up_g, 8 * t + 4)};   // heads 2t, 2t + 1
+        uint32_t qa[NT][2];
+#pragma unroll
+        for (int w = 0; w < D / 64; w++)
+#pragma unroll
+            for (int gp = 0; gp < 2; gp++)
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    const int d = 16 * (4 * w + 2 * gp) + 2 * (2 * t + c);   // a tile's element; + 16 is the group's other tile
+#pragma unroll
+                    for (int e = 0; e < 2; e++)
+                        qa[4 * w + 2 * gp + c][e] = pack2<false>(elem_to_float<DT>(qrow[d + e]) * down,
+                                                                 elem_to_float<DT>(qrow[d + 16 + e]) * down);
+                }
+
         const CodeConst cc(static_cast<uint32_t>(a.kv_heads) >> 31);
         auto compute = [&](unsigned st, uint32_t ok) {
             float sc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -421,14 +437,6 @@ q4_attend_kernel(const Args a) {
                     }
             }
         };
-        int32_t id = IDS ? fetch_id(0) : 0;
-        if (n_mine > 0) {
-#pragma unroll
-            for (int i = 0; i < R::STAGES - 1; i++) {  // tiles beyond the last copy nothing
-                issue(ring + i * R::STAGE, i, id);
-                if (IDS) id = fetch_id(i + 1);
-            }
-        }
         unsigned now = ring, next = ring + (R::STAGES - 1) * R::STAGE;
         for (int i = 0; i < n_mine; i++) {
             copy_wait<R::STAGES - 2>();
@@ -452,6 +460,7 @@ q4_attend_kernel(const Args a) {
         int per = (total + parts - 1) / parts;
         per = (per + kTile - 1) / kTile * kTile;
         const int j0 = min(total, part * per), j1 = min(total, j0 + per);
+        __syncthreads();                     // the query is in shared memory
         uint32_t qa[NT][2];
 #pragma unroll
         for (int i = 0; i < D / 32; i++) {   // lane t: elements 32 i + 8 t .. + 7 are two k-steps
@@ -555,16 +564,45 @@ q4_attend_kernel(const Args a) {
             acc += s_o[i][head][d] * f;
             sum += li * f;
         }
-        const int64_t slot = (prob * a.group + g0 + head) * a.n_split + split;
-        a.part_acc[slot * D + d] = acc;
-        if (d == 0) { a.part_ml[2 * slot] = mx; a.part_ml[2 * slot + 1] = sum; }
+        if (a.in_cluster) {   // the element this thread has just read is free
+            s_o[0][head][d] = acc;
+            if (d == 0) { s_sum[head][0] = mx; s_sum[head][1] = sum; }
+        } else {
+            const int64_t slot = (prob * a.group + g0 + head) * a.n_split + split;
+            a.part_acc[slot * D + d] = acc;
+            if (d == 0) { a.part_ml[2 * slot] = mx; a.part_ml[2 * slot + 1] = sum; }
+        }
     }
+    if (!a.in_cluster) return;
+
+    // ---- merge the CTAs of the problem through distributed shared memory, each a share of the output ----
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    const int n_cta = a.n_split;
+    for (int e = split * kThreads + tid; e < n_heads * D; e += n_cta * kThreads) {
+        const int head = e / D, d = e % D;
+        float mx = -INFINITY;
+        for (int r = 0; r < n_cta; r++) mx = fmaxf(mx, cluster.map_shared_rank(&s_sum[0][0], r)[2 * head]);
+        float acc = 0.0f, sum = 0.0f;
+        for (int r = 0; r < n_cta; r++) {
+            const float* ml = cluster.map_shared_rank(&s_sum[0][0], r);
+            const float mr = ml[2 * head], lr = ml[2 * head + 1];
+            const float ar = cluster.map_shared_rank(&s_o[0][0][0], r)[head * (D + 4) + d];
+            if (mr == -INFINITY && lr == 0.0f) continue;
+            const float f = exp2f(mr - mx);
+            acc += ar * f;
+            sum += lr * f;
+        }
+        const bool some = !(sum <= 0.0f);   // a NaN stays a NaN; nothing to attend over gives 0
+        const int64_t row = prob * a.group + g0 + head;
+        a.out[row * D + d] = float_to_elem<DT>(some ? acc / sum : 0.0f);
+        if (d == 0 && a.out_lse != nullptr) a.out_lse[row] = some ? (mx + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+    }
+    cluster.sync();   // nobody leaves while its shared memory is being read
 }
 
-// CTAs per problem (and chunk of 8 heads).  One wave of the CTAs that fit an SM; a 16-bit row costs as much as 2.7 consecutive
-// store rows or 1.6 gathered ones (115, 42 and 70 ps measured at head_dim 128); every kind of row that occurs gets at
-// least one CTA.
 constexpr int kMaxSplits = 256;
+constexpr int kMaxCluster = 8;   // the portable size
 
 template <int DT, int D, bool FEW, bool IDS>
 int launch_one(const Args& a, dim3 grid, cudaStream_t stream) {
@@ -575,7 +613,8 @@ int launch_one(const Args& a, dim3 grid, cudaStream_t stream) {
         return DC_OK;
     });
     if (rc != DC_OK) return rc;
-    DC_CUDA_TRY(launch_chained(q4_attend_kernel<DT, D, FEW, IDS>, grid, dim3(kThreads), attend_smem_bytes<D>(), stream, 0u, a));
+    DC_CUDA_TRY(launch_chained(q4_attend_kernel<DT, D, FEW, IDS>, grid, dim3(kThreads), attend_smem_bytes<D>(), stream,
+                               a.in_cluster && a.n_split > 1 ? static_cast<unsigned>(a.n_split) : 0u, a));
     return DC_OK;
 }
 
@@ -585,27 +624,41 @@ int launch(const Args& a, bool few, bool ids, dim3 grid, cudaStream_t stream) {
     return ids ? launch_one<DT, D, false, true>(a, grid, stream) : launch_one<DT, D, false, false>(a, grid, stream);
 }
 
-struct Split { int store, total; };
+// CTAs per problem (and chunk of 8 heads).  A 16-bit row costs as much as 2.7 consecutive store rows or 1.6 gathered ones
+// (115, 42 and 70 ps measured at head_dim 128); every kind of row that occurs gets at least one CTA.
+//
+// Up to 8 CTAs per problem are one cluster that finishes the output itself: one launch and no partials in memory.  That is
+// taken when 8 fill the SMs, or when the rows are so few that more CTAs would save less than the second launch costs.
+// (4096 rows of 8 problems: 10.7 us as clusters, 12.4 with partials; 8192 rows 14.0 either way.)  Otherwise the CTAs write
+// partials for a merge kernel: one wave of the CTAs that fit, or two with sequences of unequal length, whose CTAs end at
+// different times (64 problems of 0 to 32768 rows: 64.8 us with one, 49.4 with two, 56.2 with four).
+struct Split { int store, total, in_cluster; };
+constexpr int kFewUnits = 12;     // per CTA of a cluster: 768 rows
+constexpr int kRaggedWaves = 2;
 
-Split splits(int n_prob, int head_dim, bool ids, int64_t store_rows, int64_t res_rows) {
-    const int64_t target = std::max(1, ctas_per_sm(head_dim) * sm_count() / std::max(1, n_prob));
+Split splits(int n_prob, int chunks, int head_dim, bool ids, bool ragged, bool may_cluster, int64_t store_rows, int64_t res_rows) {
+    const int64_t problems = std::max<int64_t>(1, static_cast<int64_t>(n_prob) * chunks);
+    int64_t target = std::max<int64_t>(1, static_cast<int64_t>(ctas_per_sm(head_dim)) * sm_count() / problems);
     const int64_t w_store = (store_rows + 63) / 64, w_res = ((ids ? 16 : 27) * res_rows + 639) / 640;   // units of 64 store rows
-    const int64_t total = std::max<int64_t>(1, std::min<int64_t>(std::min(target, w_store + w_res), kMaxSplits - 1));
-    int64_t store = 0, res = 0;
-    if (w_store + w_res > 0) {
-        store = w_store > 0 ? std::max<int64_t>(1, (total * w_store + (w_store + w_res) / 2) / (w_store + w_res)) : 0;
-        res = w_res > 0 ? std::max<int64_t>(1, total - store) : 0;
-    }
-    if (store + res == 0) store = 1;
-    return {static_cast<int>(store), static_cast<int>(store + res)};
+    const int64_t units = std::max<int64_t>(1, w_store + w_res);
+    const bool cluster = may_cluster && ((target <= kMaxCluster && !ragged) || units <= kMaxCluster * kFewUnits);
+    if (ragged && !cluster) target = std::min(kRaggedWaves * target, (units + 3) / 4);
+    int64_t total = std::min(std::min(target, units), static_cast<int64_t>(cluster ? kMaxCluster : kMaxSplits));
+    if (w_store > 0 && w_res > 0) total = std::max<int64_t>(total, 2);
+    total = std::max<int64_t>(total, 1);
+    int64_t store = total;
+    if (w_store + w_res > 0) store = (total * w_store + (w_store + w_res) / 2) / (w_store + w_res);
+    if (w_store > 0) store = std::max<int64_t>(store, 1);
+    if (w_res > 0) store = std::min(store, total - 1);
+    return {static_cast<int>(store), static_cast<int>(total), cluster ? 1 : 0};
 }
 
 }  // namespace
 
 int64_t q4_attend_scratch_bytes(int n_prob, int group, int head_dim) {
-    // splits() makes at most ctas_per_sm * SMs / n_prob + 1 per problem (2 where that is 0 or 1), and at most kMaxSplits
+    // at most kRaggedWaves waves of CTAs, two per problem where a wave has fewer, kMaxSplits per problem
     const int64_t ctas = std::min<int64_t>(static_cast<int64_t>(n_prob) * kMaxSplits,
-                                           static_cast<int64_t>(ctas_per_sm(head_dim)) * sm_count() + 2ll * n_prob);
+                                           static_cast<int64_t>(kRaggedWaves) * ctas_per_sm(head_dim) * sm_count() + 2ll * n_prob);
     return ctas * group * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
 }
 
@@ -642,13 +695,22 @@ int q4_attend(const Q4Attend& in, cudaStream_t stream) {
     a.res_stride_b = in.res_stride_b; a.res_stride_h = in.res_stride_h;
     a.res_len = in.res_len; a.res_len_dev = in.res_len_dev;
     a.scale_log2 = (in.scale > 0.0f ? in.scale : 1.0f / std::sqrt(static_cast<float>(in.head_dim))) * kLog2e;
-    const Split sp = splits(in.n_prob, in.head_dim, in.n_sel >= 0, in.n_sel < 0 ? in.n_rows : in.n_sel, in.res_len + (in.k_new ? 1 : 0));
+    const int chunks = (in.group + kHeads - 1) / kHeads;
+    const Split sp = splits(in.n_prob, chunks, in.head_dim, in.n_sel >= 0, in.n_sel < 0 && in.lens != nullptr,
+                            in.out != nullptr && in.xout == nullptr && in.fin == nullptr, in.n_sel < 0 ? in.n_rows : in.n_sel,
+                            in.res_len + (in.k_new ? 1 : 0));
     a.n_store_split = sp.store;
     a.n_split = sp.total;
+    a.in_cluster = sp.in_cluster;
+    DC_REQUIRE(a.in_cluster || static_cast<int64_t>(in.n_prob) * a.n_split * in.group * (in.head_dim + 2) * 4 <=
+                                   q4_attend_scratch_bytes(in.n_prob, in.group, in.head_dim),
+               "q4_attend: %d partials per problem exceed the scratch buffer", a.n_split);
+    a.out = static_cast<uint16_t*>(in.out);
+    a.out_lse = in.out_lse;
     a.part_acc = static_cast<float*>(in.scratch);
     a.part_ml = a.part_acc + static_cast<int64_t>(in.n_prob) * a.n_split * in.group * in.head_dim;
     const dim3 grid(static_cast<unsigned>(a.n_split), static_cast<unsigned>(in.n_prob),
-                    static_cast<unsigned>((in.group + kHeads - 1) / kHeads));
+                    static_cast<unsigned>(chunks));
 #define CASE(DT, D) rc = launch<DT, D>(a, in.group <= 4, in.n_sel >= 0, grid, stream)
     int rc = DC_OK;
     if (in.dtype == DC_BF16) {
@@ -661,7 +723,7 @@ int q4_attend(const Q4Attend& in, cudaStream_t stream) {
         else { CASE(DC_FP16, 256); }
     }
 #undef CASE
-    if (rc != DC_OK) return rc;
+    if (rc != DC_OK || a.in_cluster) return rc;
     return lse_combine(a.part_acc, in.head_dim, static_cast<int64_t>(a.n_split) * in.head_dim, a.part_ml, 2,
                        static_cast<int64_t>(a.n_split) * 2, a.n_split, static_cast<int64_t>(in.n_prob) * in.group, in.head_dim,
                        in.dtype, in.out, in.out_lse, in.out_acc, in.out_ml, stream, nullptr, in.xout, in.fin, true);
