@@ -49,11 +49,11 @@ struct Args {
     float scale_log2;
     int n_store_split;               // CTAs (per problem and head chunk) that take store rows; the others take 16-bit rows
     int n_split;
-    int in_cluster;                  // the n_split CTAs of a problem are one cluster and finish the output themselves
-    uint16_t* out;                   // then: (n_prob, group, D) and optional (n_prob, group)
+    int cluster;                     // that many consecutive CTAs of a problem are one cluster and merge their results
+    uint16_t* out;                   // set where one cluster is all there is: (n_prob, group, D), and optional (n_prob, group)
     float* out_lse;
-    float* part_acc;                 // otherwise: (n_prob, group, n_split, D)
-    float* part_ml;                  // (n_prob, group, n_split, 2)
+    float* part_acc;                 // otherwise: (n_prob, group, n_split / cluster, D)
+    float* part_ml;                  // (n_prob, group, n_split / cluster, 2)
 };
 
 // ---- a tile of 16 store rows in shared memory, private to one warp ----
@@ -228,9 +228,8 @@ q4_attend_kernel(const Args a) {
 
     if (split < a.n_store_split) {
         const int64_t n_rows = a.n_rows_dev != nullptr ? min(a.n_rows, static_cast<int64_t>(*a.n_rows_dev)) : a.n_rows;
-        const uint32_t* sel = IDS ? a.sel + prob * a.sel_stride : nullptr;
         // rows of the store: the first sel_count ids of the list, or rows 0 .. lens[b] - 1
-        int64_t n_store = IDS ? (n_rows > 0 ? a.n_sel : 0) : n_rows;
+        int64_t n_store = IDS ? a.n_sel : n_rows;
         if (IDS && a.sel_count) n_store = max(static_cast<int64_t>(0), min(n_store, static_cast<int64_t>(a.sel_count[prob])));
         if (!IDS && a.lens) n_store = max(static_cast<int64_t>(0), min(n_rows, static_cast<int64_t>(a.lens[b])));
         int64_t per = (n_store + a.n_store_split - 1) / a.n_store_split;
@@ -249,16 +248,17 @@ q4_attend_kernel(const Args a) {
 #pragma unroll
         for (int j = 0; j < NC; j++) dst[j] = R::chunk((lane + 32 * j) / CPR, (lane + 32 * j) % CPR);
         const int dst_scale = 2 * R::CODES + lane * (D / 16);
-        // This lane's row of a tile's 16 (lane and lane + 16 hold the same); -1 where there is none.
-        auto fetch_id = [&](int i) -> int32_t {
+        // This lane's id of a tile's 16 (lane and lane + 16 hold the same), as listed, and as a row: -1 where there is none.
+        // sel_base + n_rows < 2^32 (checked on the host), so pads and ids of other shards end up beyond n_rows.
+        auto listed_id = [&](int i) -> uint32_t {
             const int64_t j = j0 + (warp + static_cast<int64_t>(i) * kWarps) * kTile + (lane & 15);
-            if (j >= j1) return -1;
-            const int64_t row = static_cast<int64_t>(sel[j]) - a.sel_base;
-            return row >= 0 && row < n_rows ? static_cast<int32_t>(row) : -1;   // pads and ids of other shards
+            return j < j1 ? a.sel[prob * a.sel_stride + j] - static_cast<uint32_t>(a.sel_base) : 0xFFFFFFFFu;
         };
+        auto row_of = [&](uint32_t id) -> int32_t { return id < n_rows ? static_cast<int32_t>(id) : -1; };
         // Consecutive rows: 16 of them are one run of bytes per array, so the addresses just advance from tile to tile.
-        const uint8_t* kp = kc + (j0 + warp * kTile) * (D / 2) + lane * 16;
-        const uint8_t* vp = vc + (j0 + warp * kTile) * (D / 2) + lane * 16;
+        // (ids: this lane's chunk of any row is a multiple of the row length away.)
+        const uint8_t* kp = kc + (IDS ? lane % CPR * 16 : (j0 + warp * kTile) * (D / 2) + lane * 16);
+        const uint8_t* vp = vc + (IDS ? lane % CPR * 16 : (j0 + warp * kTile) * (D / 2) + lane * 16);
         const uint8_t* sp = sc_base + (j0 + warp * kTile + (lane & 15)) * (D / 16);
         const int n_mine = static_cast<int>((max(j1 - j0 - warp * kTile, static_cast<int64_t>(0)) + kWarps * kTile - 1) / (kWarps * kTile));
         const int last_rows = static_cast<int>(j1 - j0) - (warp + (n_mine - 1) * kWarps) * kTile;   // of this warp's last tile; > 16: whole
@@ -285,16 +285,24 @@ q4_attend_kernel(const Args a) {
                 vp += kWarps * kTile * (D / 2);
                 sp += kWarps * kTile * (D / 16);
             } else {
+                const uint32_t ok = __ballot_sync(0xFFFFFFFFu, id >= 0);
+                const uint32_t safe = max(id, 0);      // (nothing is read where there is no row)
+                const uint8_t* sc_at = sc_base + static_cast<uint64_t>(safe) * (D / 16);
 #pragma unroll
                 for (int j = 0; j < NC; j++) {
-                    const int32_t row = __shfl_sync(0xFFFFFFFFu, id, (lane + 32 * j) / CPR);
-                    const int64_t off = max(row, 0) * static_cast<int64_t>(D / 2) + (lane + 32 * j) % CPR * 16;
-                    copy_async<16>(st + dst[j], kc + off, row >= 0);
-                    copy_async<16>(st + R::CODES + dst[j], vc + off, row >= 0);
+                    const uint64_t off = static_cast<uint64_t>(__shfl_sync(0xFFFFFFFFu, safe, (lane + 32 * j) / CPR)) * (D / 2);
+                    if (ok == 0xFFFFFFFFu) {
+                        copy_async<16>(st + dst[j], kp + off);
+                        copy_async<16>(st + R::CODES + dst[j], vp + off);
+                    } else {
+                        const bool there = (ok >> ((lane + 32 * j) / CPR)) & 1u;
+                        copy_async<16>(st + dst[j], kp + off, there);
+                        copy_async<16>(st + R::CODES + dst[j], vp + off, there);
+                    }
                 }
-                copy_async<D / 16>(st + dst_scale, sc_base + max(id, 0) * static_cast<int64_t>(D / 16), id >= 0);
-                const uint32_t ok = __ballot_sync(0xFFFFFFFFu, id >= 0) & 0xFFFFu;
-                if (lane == 0) s_ok[warp][i % R::STAGES] = ok;
+                if (ok == 0xFFFFFFFFu) copy_async<D / 16>(st + dst_scale, sc_at);
+                else copy_async<D / 16>(st + dst_scale, sc_at, id >= 0);
+                if (lane == 0) s_ok[warp][i % R::STAGES] = ok & 0xFFFFu;
             }
             copy_commit();
         };
@@ -309,14 +317,16 @@ q4_attend_kernel(const Args a) {
 #pragma unroll
         for (int i = 0; i < 4; i++)
             v_at[i] = R::CODES + R::chunk(4 * t + i, g * (D / 16) / 16) + g * (D / 16) % 16;
-        int32_t id = IDS ? fetch_id(0) : 0;
+        uint32_t id[R::STAGES] = {};                   // of the first tiles; then id[0] runs one tile ahead of the copies
+        if (IDS) {
+#pragma unroll
+            for (int i = 0; i < R::STAGES; i++) id[i] = listed_id(i);
+        }
         if (n_mine > 0) {
 #pragma unroll
-            for (int i = 0; i < R::STAGES - 1; i++) {  // tiles beyond the last copy nothing
-                issue(ring + i * R::STAGE, i, id);
-                if (IDS) id = fetch_id(i + 1);
-            }
+            for (int i = 0; i < R::STAGES - 1; i++) issue(ring + i * R::STAGE, i, IDS ? row_of(id[i]) : 0);   // beyond the last: nothing
         }
+        id[0] = id[R::STAGES - 1];
         __syncthreads();                               // the query is in shared memory
         // query fragments, normalised to [2^14, 2^15) by a power of two
         float top = 0.0f;
@@ -441,8 +451,8 @@ q4_attend_kernel(const Args a) {
         for (int i = 0; i < n_mine; i++) {
             copy_wait<R::STAGES - 2>();
             __syncwarp();   // every lane's copies of this tile have landed, and nobody reads the tile before any more
-            issue(next, i + R::STAGES - 1, id);
-            if (IDS) id = fetch_id(i + R::STAGES);
+            issue(next, i + R::STAGES - 1, IDS ? row_of(id[0]) : 0);
+            if (IDS) id[0] = listed_id(i + R::STAGES);
             compute(now, IDS ? s_ok[warp][i % R::STAGES] : i < n_mine - 1 || last_rows >= kTile ? 0xFFFFu : (1u << last_rows) - 1u);
             next = now;
             now = now == ring + (R::STAGES - 1) * R::STAGE ? ring : now + R::STAGE;
@@ -564,44 +574,108 @@ q4_attend_kernel(const Args a) {
             acc += s_o[i][head][d] * f;
             sum += li * f;
         }
-        if (a.in_cluster) {   // the element this thread has just read is free
-            s_o[0][head][d] = acc;
-            if (d == 0) { s_sum[head][0] = mx; s_sum[head][1] = sum; }
-        } else {
+        if (a.out == nullptr && a.cluster == 1) {
             const int64_t slot = (prob * a.group + g0 + head) * a.n_split + split;
             a.part_acc[slot * D + d] = acc;
             if (d == 0) { a.part_ml[2 * slot] = mx; a.part_ml[2 * slot + 1] = sum; }
+        } else {
+            s_o[0][head][d] = acc;           // the element this thread has just read is free
+            if (d == 0) { s_sum[head][0] = mx; s_sum[head][1] = sum; }
         }
     }
-    if (!a.in_cluster) return;
+    if (a.out == nullptr && a.cluster == 1) return;
 
-    // ---- merge the CTAs of the problem through distributed shared memory, each a share of the output ----
+    // ---- merge the CTAs of the cluster through distributed shared memory, each a share of the elements ----
     cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync();
-    const int n_cta = a.n_split;
-    for (int e = split * kThreads + tid; e < n_heads * D; e += n_cta * kThreads) {
+    if (a.cluster > 1) cluster.sync();
+    else __syncthreads();
+    const int n_part = a.n_split / a.cluster, part = split / a.cluster;
+    for (int e = (split % a.cluster) * kThreads + tid; e < n_heads * D; e += a.cluster * kThreads) {
         const int head = e / D, d = e % D;
         float mx = -INFINITY;
-        for (int r = 0; r < n_cta; r++) mx = fmaxf(mx, cluster.map_shared_rank(&s_sum[0][0], r)[2 * head]);
+        for (int r = 0; r < a.cluster; r++) mx = fmaxf(mx, cluster.map_shared_rank(&s_sum[0][0], r)[2 * head]);
         float acc = 0.0f, sum = 0.0f;
-        for (int r = 0; r < n_cta; r++) {
+        for (int r = 0; r < a.cluster; r++) {
             const float* ml = cluster.map_shared_rank(&s_sum[0][0], r);
             const float mr = ml[2 * head], lr = ml[2 * head + 1];
             const float ar = cluster.map_shared_rank(&s_o[0][0][0], r)[head * (D + 4) + d];
-            if (mr == -INFINITY && lr == 0.0f) continue;
+            if (mr == -INFINITY && lr == 0.0f) continue;   // a CTA without rows
             const float f = exp2f(mr - mx);
             acc += ar * f;
             sum += lr * f;
         }
-        const bool some = !(sum <= 0.0f);   // a NaN stays a NaN; nothing to attend over gives 0
         const int64_t row = prob * a.group + g0 + head;
-        a.out[row * D + d] = float_to_elem<DT>(some ? acc / sum : 0.0f);
-        if (d == 0 && a.out_lse != nullptr) a.out_lse[row] = some ? (mx + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+        if (a.out != nullptr) {
+            const bool some = !(sum <= 0.0f);   // a NaN stays a NaN; nothing to attend over gives 0
+            a.out[row * D + d] = float_to_elem<DT>(some ? acc / sum : 0.0f);
+            if (d == 0 && a.out_lse != nullptr) a.out_lse[row] = some ? (mx + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+        } else {
+            const int64_t slot = row * n_part + part;
+            a.part_acc[slot * D + d] = acc;
+            if (d == 0) { a.part_ml[2 * slot] = mx; a.part_ml[2 * slot + 1] = sum; }
+        }
     }
-    cluster.sync();   // nobody leaves while its shared memory is being read
+    if (a.cluster > 1) cluster.sync();   // nobody leaves while its shared memory is being read
 }
 
 constexpr int kMaxSplits = 256;
+
+// Merge of n_part partials per row into the output: grid = (rows, D / 64), a CTA has 64 elements of a row, 16 lanes of four
+// elements by 16 groups of parts.
+constexpr int kMergeThreads = 256;
+
+template <int DT>
+__global__ void __launch_bounds__(kMergeThreads)
+q4_merge_kernel(const float* __restrict__ part_acc, const float* __restrict__ part_ml, int n_part, int dim,
+                uint16_t* __restrict__ out, float* __restrict__ out_lse) {
+    pdl_launch_dependents();
+    pdl_wait();
+    __shared__ float s_w[kMaxSplits];
+    __shared__ float s_red[2][kMergeThreads / 32];
+    __shared__ __align__(16) float4 s_acc[16][16];
+    const int64_t row = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = tid & 15, grp = tid >> 4;
+    // thread i has part i: its (reference, sum)
+    const float2 ml = tid < n_part ? reinterpret_cast<const float2*>(part_ml)[row * n_part + tid] : make_float2(-INFINITY, 0.0f);
+    const bool has = !(ml.x == -INFINITY && ml.y == 0.0f);
+    float mx = ml.x;
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, off));
+    if (lane == 0) s_red[0][warp] = mx;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kMergeThreads / 32; i++) mx = fmaxf(mx, s_red[0][i]);
+    const float w = has ? exp2f(ml.x - mx) : 0.0f;
+    if (tid < n_part) s_w[tid] = w;
+    float sum = has ? ml.y * w : 0.0f;
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, off);
+    if (lane == 0) s_red[1][warp] = sum;
+    __syncthreads();
+    sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kMergeThreads / 32; i++) sum += s_red[1][i];
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const float* src = part_acc + (row * n_part) * dim + blockIdx.y * 64 + 4 * c;
+#pragma unroll 4
+    for (int i = grp; i < n_part; i += 16) {
+        const float4 v = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(i) * dim);
+        const float f = s_w[i];
+        acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+    }
+    s_acc[grp][c] = acc;
+    __syncthreads();
+    if (tid < 64) {
+        const float* col = reinterpret_cast<const float*>(s_acc) + tid;
+        float v = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; i++) v += col[64 * i];
+        const bool some = !(sum <= 0.0f);   // a NaN stays a NaN; nothing to attend over gives 0
+        out[row * dim + blockIdx.y * 64 + tid] = float_to_elem<DT>(some ? v / sum : 0.0f);
+        if (tid == 0 && blockIdx.y == 0 && out_lse != nullptr)
+            out_lse[row] = some ? (mx + log2f(sum)) * 0.6931471805599453f : -INFINITY;
+    }
+}
 constexpr int kMaxCluster = 8;   // the portable size
 
 template <int DT, int D, bool FEW, bool IDS>
@@ -614,7 +688,7 @@ int launch_one(const Args& a, dim3 grid, cudaStream_t stream) {
     });
     if (rc != DC_OK) return rc;
     DC_CUDA_TRY(launch_chained(q4_attend_kernel<DT, D, FEW, IDS>, grid, dim3(kThreads), attend_smem_bytes<D>(), stream,
-                               a.in_cluster && a.n_split > 1 ? static_cast<unsigned>(a.n_split) : 0u, a));
+                               a.cluster > 1 ? static_cast<unsigned>(a.cluster) : 0u, a));
     return DC_OK;
 }
 
@@ -627,39 +701,41 @@ int launch(const Args& a, bool few, bool ids, dim3 grid, cudaStream_t stream) {
 // CTAs per problem (and chunk of 8 heads).  A 16-bit row costs as much as 2.7 consecutive store rows or 1.6 gathered ones
 // (115, 42 and 70 ps measured at head_dim 128); every kind of row that occurs gets at least one CTA.
 //
-// Up to 8 CTAs per problem are one cluster that finishes the output itself: one launch and no partials in memory.  That is
-// taken when 8 fill the SMs, or when the rows are so few that more CTAs would save less than the second launch costs.
-// (4096 rows of 8 problems: 10.7 us as clusters, 12.4 with partials; 8192 rows 14.0 either way.)  Otherwise the CTAs write
-// partials for a merge kernel: one wave of the CTAs that fit, or two with sequences of unequal length, whose CTAs end at
-// different times (64 problems of 0 to 32768 rows: 64.8 us with one, 49.4 with two, 56.2 with four).
-struct Split { int store, total, in_cluster; };
+// Up to 8 CTAs of a problem are a cluster that merges its results on chip and finishes the output, in one launch; that is
+// taken when 8 CTAs per problem fill the SMs, or when the rows are so few that more CTAs would save less than the second
+// launch costs (4096 rows of 8 problems: 10.7 us in one launch, 12.4 in two; 8192 rows 14.0 either way).  Otherwise every
+// CTA writes a partial for a merge kernel: one wave of the CTAs that fit, or two with sequences of unequal length, whose
+// CTAs end at different times (64 problems of 0 to 32768 rows: 64.8 us with one, 49.4 with two, 56.2 with four).  Clusters
+// of 8 in those launches as well would merge on chip first, but do not fill every SM: 4 x 65536 rows of head_dim 256 took
+// 54 us with them, 36 without.
+struct Split { int store, total, cluster; };
 constexpr int kFewUnits = 12;     // per CTA of a cluster: 768 rows
 constexpr int kRaggedWaves = 2;
 
-Split splits(int n_prob, int chunks, int head_dim, bool ids, bool ragged, bool may_cluster, int64_t store_rows, int64_t res_rows) {
+Split splits(int n_prob, int chunks, int head_dim, bool ids, bool ragged, int64_t store_rows, int64_t res_rows) {
     const int64_t problems = std::max<int64_t>(1, static_cast<int64_t>(n_prob) * chunks);
     int64_t target = std::max<int64_t>(1, static_cast<int64_t>(ctas_per_sm(head_dim)) * sm_count() / problems);
     const int64_t w_store = (store_rows + 63) / 64, w_res = ((ids ? 16 : 27) * res_rows + 639) / 640;   // units of 64 store rows
     const int64_t units = std::max<int64_t>(1, w_store + w_res);
-    const bool cluster = may_cluster && ((target <= kMaxCluster && !ragged) || units <= kMaxCluster * kFewUnits);
-    if (ragged && !cluster) target = std::min(kRaggedWaves * target, (units + 3) / 4);
-    int64_t total = std::min(std::min(target, units), static_cast<int64_t>(cluster ? kMaxCluster : kMaxSplits));
+    const bool one = (target <= kMaxCluster && !ragged) || units <= kMaxCluster * kFewUnits;
+    if (ragged && !one) target = std::min(kRaggedWaves * target, (units + 3) / 4);
+    int64_t total = std::min(std::min(target, units), static_cast<int64_t>(one ? kMaxCluster : kMaxSplits));
     if (w_store > 0 && w_res > 0) total = std::max<int64_t>(total, 2);
     total = std::max<int64_t>(total, 1);
     int64_t store = total;
     if (w_store + w_res > 0) store = (total * w_store + (w_store + w_res) / 2) / (w_store + w_res);
     if (w_store > 0) store = std::max<int64_t>(store, 1);
     if (w_res > 0) store = std::min(store, total - 1);
-    return {static_cast<int>(store), static_cast<int>(total), cluster ? 1 : 0};
+    return {static_cast<int>(store), static_cast<int>(total), total <= kMaxCluster ? static_cast<int>(total) : 1};
 }
 
 }  // namespace
 
 int64_t q4_attend_scratch_bytes(int n_prob, int group, int head_dim) {
-    // at most kRaggedWaves waves of CTAs, two per problem where a wave has fewer, kMaxSplits per problem
-    const int64_t ctas = std::min<int64_t>(static_cast<int64_t>(n_prob) * kMaxSplits,
-                                           static_cast<int64_t>(kRaggedWaves) * ctas_per_sm(head_dim) * sm_count() + 2ll * n_prob);
-    return ctas * group * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
+    // at most kRaggedWaves waves of CTAs, one cluster per problem where a wave has fewer, kMaxSplits per problem
+    const int64_t parts = std::min<int64_t>(static_cast<int64_t>(n_prob) * kMaxSplits,
+                                            static_cast<int64_t>(kRaggedWaves) * ctas_per_sm(head_dim) * sm_count() + n_prob);
+    return parts * group * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
 }
 
 int q4_attend(const Q4Attend& in, cudaStream_t stream) {
@@ -670,6 +746,8 @@ int q4_attend(const Q4Attend& in, cudaStream_t stream) {
     DC_REQUIRE(in.res_len >= 0, "q4_attend: negative length");
     DC_REQUIRE(in.n_sel <= 0 || (in.sel != nullptr && in.sel_stride >= in.n_sel), "q4_attend: n_sel=%d without ids, or sel_stride=%lld",
                in.n_sel, static_cast<long long>(in.sel_stride));
+    DC_REQUIRE(in.sel_base >= 0 && in.sel_base + in.n_rows < (1ll << 32), "q4_attend: sel_base=%lld: ids are 32 bits",
+               static_cast<long long>(in.sel_base));
     DC_REQUIRE((in.k_new == nullptr) == (in.v_new == nullptr), "q4_attend: k_new and v_new must both be set or both be NULL");
     DC_REQUIRE((in.res_k == nullptr) == (in.res_v == nullptr), "q4_attend: res_k and res_v must both be set or both be NULL");
     DC_REQUIRE(in.res_len == 0 || in.res_k != nullptr, "q4_attend: res_len > 0 needs resident buffers");
@@ -697,18 +775,19 @@ int q4_attend(const Q4Attend& in, cudaStream_t stream) {
     a.scale_log2 = (in.scale > 0.0f ? in.scale : 1.0f / std::sqrt(static_cast<float>(in.head_dim))) * kLog2e;
     const int chunks = (in.group + kHeads - 1) / kHeads;
     const Split sp = splits(in.n_prob, chunks, in.head_dim, in.n_sel >= 0, in.n_sel < 0 && in.lens != nullptr,
-                            in.out != nullptr && in.xout == nullptr && in.fin == nullptr, in.n_sel < 0 ? in.n_rows : in.n_sel,
-                            in.res_len + (in.k_new ? 1 : 0));
+                            in.n_sel < 0 ? in.n_rows : in.n_sel, in.res_len + (in.k_new ? 1 : 0));
+    const int n_part = sp.total / sp.cluster;
+    const bool finish = n_part == 1 && in.out != nullptr && in.xout == nullptr && in.fin == nullptr;
     a.n_store_split = sp.store;
     a.n_split = sp.total;
-    a.in_cluster = sp.in_cluster;
-    DC_REQUIRE(a.in_cluster || static_cast<int64_t>(in.n_prob) * a.n_split * in.group * (in.head_dim + 2) * 4 <=
-                                   q4_attend_scratch_bytes(in.n_prob, in.group, in.head_dim),
-               "q4_attend: %d partials per problem exceed the scratch buffer", a.n_split);
-    a.out = static_cast<uint16_t*>(in.out);
+    a.cluster = sp.cluster;
+    a.out = finish ? static_cast<uint16_t*>(in.out) : nullptr;
     a.out_lse = in.out_lse;
+    DC_REQUIRE(finish || static_cast<int64_t>(in.n_prob) * n_part * in.group * (in.head_dim + 2) * 4 <=
+                             q4_attend_scratch_bytes(in.n_prob, in.group, in.head_dim),
+               "q4_attend: %d partials per problem exceed the scratch buffer", n_part);
     a.part_acc = static_cast<float*>(in.scratch);
-    a.part_ml = a.part_acc + static_cast<int64_t>(in.n_prob) * a.n_split * in.group * in.head_dim;
+    a.part_ml = a.part_acc + static_cast<int64_t>(in.n_prob) * n_part * in.group * in.head_dim;
     const dim3 grid(static_cast<unsigned>(a.n_split), static_cast<unsigned>(in.n_prob),
                     static_cast<unsigned>(chunks));
 #define CASE(DT, D) rc = launch<DT, D>(a, in.group <= 4, in.n_sel >= 0, grid, stream)
@@ -723,9 +802,19 @@ int q4_attend(const Q4Attend& in, cudaStream_t stream) {
         else { CASE(DC_FP16, 256); }
     }
 #undef CASE
-    if (rc != DC_OK || a.in_cluster) return rc;
-    return lse_combine(a.part_acc, in.head_dim, static_cast<int64_t>(a.n_split) * in.head_dim, a.part_ml, 2,
-                       static_cast<int64_t>(a.n_split) * 2, a.n_split, static_cast<int64_t>(in.n_prob) * in.group, in.head_dim,
+    if (rc != DC_OK || finish) return rc;
+    if (in.out != nullptr && in.xout == nullptr && in.fin == nullptr) {
+        const dim3 merge(static_cast<unsigned>(in.n_prob * in.group), static_cast<unsigned>(in.head_dim / 64));
+        if (in.dtype == DC_BF16)
+            DC_CUDA_TRY(launch_chained(q4_merge_kernel<DC_BF16>, merge, dim3(kMergeThreads), 0, stream, 0u, a.part_acc, a.part_ml,
+                                       n_part, in.head_dim, static_cast<uint16_t*>(in.out), in.out_lse));
+        else
+            DC_CUDA_TRY(launch_chained(q4_merge_kernel<DC_FP16>, merge, dim3(kMergeThreads), 0, stream, 0u, a.part_acc, a.part_ml,
+                                       n_part, in.head_dim, static_cast<uint16_t*>(in.out), in.out_lse));
+        return DC_OK;
+    }
+    return lse_combine(a.part_acc, in.head_dim, static_cast<int64_t>(n_part) * in.head_dim, a.part_ml, 2,
+                       static_cast<int64_t>(n_part) * 2, n_part, static_cast<int64_t>(in.n_prob) * in.group, in.head_dim,
                        in.dtype, in.out, in.out_lse, in.out_acc, in.out_ml, stream, nullptr, in.xout, in.fin, true);
 }
 
