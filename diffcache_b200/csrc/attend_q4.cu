@@ -49,6 +49,7 @@ struct Args {
     float scale_log2;
     int n_store_split;               // CTAs (per problem and head chunk) that take store rows; the others take 16-bit rows
     int n_split;
+    int64_t run;                     // rows of the store a CTA takes; 0: an equal share of the problem's rows
     int cluster;                     // that many consecutive CTAs of a problem are one cluster and merge their results
     uint16_t* out;                   // set where one cluster is all there is: (n_prob, group, D), and optional (n_prob, group)
     float* out_lse;
@@ -232,9 +233,17 @@ q4_attend_kernel(const Args a) {
         int64_t n_store = IDS ? a.n_sel : n_rows;
         if (IDS && a.sel_count) n_store = max(static_cast<int64_t>(0), min(n_store, static_cast<int64_t>(a.sel_count[prob])));
         if (!IDS && a.lens) n_store = max(static_cast<int64_t>(0), min(n_rows, static_cast<int64_t>(a.lens[b])));
-        int64_t per = (n_store + a.n_store_split - 1) / a.n_store_split;
-        per = (per + kTile - 1) / kTile * kTile;
+        int64_t per = a.run;
+        if (per == 0) per = ((n_store + a.n_store_split - 1) / a.n_store_split + kTile - 1) / kTile * kTile;
         const int64_t j0 = min(n_store, split * per), j1 = min(n_store, j0 + per);
+        if (a.run != 0 && j0 >= j1) {   // a run behind the end of this sequence: an empty partial, whose sums are not read
+            if (tid < n_heads) {
+                float* ml = a.part_ml + 2 * ((prob * a.group + g0 + tid) * a.n_split + split);
+                ml[0] = -INFINITY;
+                ml[1] = 0.0f;
+            }
+            return;
+        }
         const uint8_t* kc = a.st.k.codes + prob * a.st.prob_rows * (D / 2);
         const uint8_t* vc = a.st.v.codes + prob * a.st.prob_rows * (D / 2);
         const uint8_t* sc_base = reinterpret_cast<const uint8_t*>((lane < 16 ? a.st.k.scales : a.st.v.scales) + prob * a.st.prob_rows * NG);
@@ -661,6 +670,7 @@ q4_merge_kernel(const float* __restrict__ part_acc, const float* __restrict__ pa
     for (int i = grp; i < n_part; i += 16) {
         const float4 v = *reinterpret_cast<const float4*>(src + static_cast<int64_t>(i) * dim);
         const float f = s_w[i];
+        if (f == 0.0f) continue;   // an empty partial, or one that does not count
         acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
     }
     s_acc[grp][c] = acc;
@@ -704,13 +714,16 @@ int launch(const Args& a, bool few, bool ids, dim3 grid, cudaStream_t stream) {
 // Up to 8 CTAs of a problem are a cluster that merges its results on chip and finishes the output, in one launch; that is
 // taken when 8 CTAs per problem fill the SMs, or when the rows are so few that more CTAs would save less than the second
 // launch costs (4096 rows of 8 problems: 10.7 us in one launch, 12.4 in two; 8192 rows 14.0 either way).  Otherwise every
-// CTA writes a partial for a merge kernel: one wave of the CTAs that fit, or two with sequences of unequal length, whose
-// CTAs end at different times (64 problems of 0 to 32768 rows: 64.8 us with one, 49.4 with two, 56.2 with four).  Clusters
+// CTA writes a partial for a merge kernel: one wave of the CTAs that fit.  With sequences of unequal length a CTA takes a
+// run of the same length whatever its sequence (shares of each sequence took 66 us instead of 52 on 64 problems of 0 to
+// 32768 rows), runs behind a sequence's end exit at once, and there are two waves of them (one: 65 us), up to eight as long
+// as a run keeps 2048 rows (128 problems of 0 to 131072 rows: 405 us with two, 336 with eight).  Clusters
 // of 8 in those launches as well would merge on chip first, but do not fill every SM: 4 x 65536 rows of head_dim 256 took
 // 54 us with them, 36 without.
-struct Split { int store, total, cluster; };
+struct Split { int store, total, cluster; int64_t run; };
 constexpr int kFewUnits = 12;     // per CTA of a cluster: 768 rows
-constexpr int kRaggedWaves = 2;
+constexpr int kMaxWaves = 8;
+constexpr int kWaveUnits = 32;    // 2048 rows
 
 Split splits(int n_prob, int chunks, int head_dim, bool ids, bool ragged, int64_t store_rows, int64_t res_rows) {
     const int64_t problems = std::max<int64_t>(1, static_cast<int64_t>(n_prob) * chunks);
@@ -718,7 +731,10 @@ Split splits(int n_prob, int chunks, int head_dim, bool ids, bool ragged, int64_
     const int64_t w_store = (store_rows + 63) / 64, w_res = ((ids ? 16 : 27) * res_rows + 639) / 640;   // units of 64 store rows
     const int64_t units = std::max<int64_t>(1, w_store + w_res);
     const bool one = (target <= kMaxCluster && !ragged) || units <= kMaxCluster * kFewUnits;
-    if (ragged && !one) target = std::min(kRaggedWaves * target, (units + 3) / 4);
+    if (ragged && !one) {
+        const int64_t waves = std::max<int64_t>(2, std::min<int64_t>(kMaxWaves, units / target / kWaveUnits));
+        target = std::min(waves * target, (units + 3) / 4);
+    }
     int64_t total = std::min(std::min(target, units), static_cast<int64_t>(one ? kMaxCluster : kMaxSplits));
     if (w_store > 0 && w_res > 0) total = std::max<int64_t>(total, 2);
     total = std::max<int64_t>(total, 1);
@@ -726,15 +742,16 @@ Split splits(int n_prob, int chunks, int head_dim, bool ids, bool ragged, int64_
     if (w_store + w_res > 0) store = (total * w_store + (w_store + w_res) / 2) / (w_store + w_res);
     if (w_store > 0) store = std::max<int64_t>(store, 1);
     if (w_res > 0) store = std::min(store, total - 1);
-    return {static_cast<int>(store), static_cast<int>(total), total <= kMaxCluster ? static_cast<int>(total) : 1};
+    return {static_cast<int>(store), static_cast<int>(total), total <= kMaxCluster ? static_cast<int>(total) : 1,
+            ragged && total > kMaxCluster ? ((store_rows + store - 1) / store + kTile - 1) / kTile * kTile : 0};
 }
 
 }  // namespace
 
 int64_t q4_attend_scratch_bytes(int n_prob, int group, int head_dim) {
-    // at most kRaggedWaves waves of CTAs, one cluster per problem where a wave has fewer, kMaxSplits per problem
+    // at most kMaxWaves waves of CTAs, one cluster per problem where a wave has fewer, kMaxSplits per problem
     const int64_t parts = std::min<int64_t>(static_cast<int64_t>(n_prob) * kMaxSplits,
-                                            static_cast<int64_t>(kRaggedWaves) * ctas_per_sm(head_dim) * sm_count() + n_prob);
+                                            static_cast<int64_t>(kMaxWaves) * ctas_per_sm(head_dim) * sm_count() + n_prob);
     return parts * group * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
 }
 
@@ -774,13 +791,16 @@ int q4_attend(const Q4Attend& in, cudaStream_t stream) {
     a.res_len = in.res_len; a.res_len_dev = in.res_len_dev;
     a.scale_log2 = (in.scale > 0.0f ? in.scale : 1.0f / std::sqrt(static_cast<float>(in.head_dim))) * kLog2e;
     const int chunks = (in.group + kHeads - 1) / kHeads;
-    const Split sp = splits(in.n_prob, chunks, in.head_dim, in.n_sel >= 0, in.n_sel < 0 && in.lens != nullptr,
+    // the exchanges and callers of partials take the merge of attend.cu, which reads every partial: no empty runs there
+    const bool own_merge = in.out != nullptr && in.xout == nullptr && in.fin == nullptr;
+    const Split sp = splits(in.n_prob, chunks, in.head_dim, in.n_sel >= 0, own_merge && in.n_sel < 0 && in.lens != nullptr,
                             in.n_sel < 0 ? in.n_rows : in.n_sel, in.res_len + (in.k_new ? 1 : 0));
     const int n_part = sp.total / sp.cluster;
-    const bool finish = n_part == 1 && in.out != nullptr && in.xout == nullptr && in.fin == nullptr;
+    const bool finish = n_part == 1 && own_merge;
     a.n_store_split = sp.store;
     a.n_split = sp.total;
     a.cluster = sp.cluster;
+    a.run = sp.run;
     a.out = finish ? static_cast<uint16_t*>(in.out) : nullptr;
     a.out_lse = in.out_lse;
     DC_REQUIRE(finish || static_cast<int64_t>(in.n_prob) * n_part * in.group * (in.head_dim + 2) * 4 <=
@@ -803,7 +823,7 @@ int q4_attend(const Q4Attend& in, cudaStream_t stream) {
     }
 #undef CASE
     if (rc != DC_OK || finish) return rc;
-    if (in.out != nullptr && in.xout == nullptr && in.fin == nullptr) {
+    if (own_merge) {
         const dim3 merge(static_cast<unsigned>(in.n_prob * in.group), static_cast<unsigned>(in.head_dim / 64));
         if (in.dtype == DC_BF16)
             DC_CUDA_TRY(launch_chained(q4_merge_kernel<DC_BF16>, merge, dim3(kMergeThreads), 0, stream, 0u, a.part_acc, a.part_ml,

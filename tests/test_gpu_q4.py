@@ -683,6 +683,52 @@ def test_stateless_functions_equal_the_engine():
     assert torch.equal(o1, o2)
 
 
+@pytest.mark.parametrize("partials", [False, True])
+def test_ragged_runs_never_read_what_nobody_wrote(partials):
+    """Long unequal sequences through the stateless call with a scratch buffer full of NaN, as output and as partials."""
+    from diffcache_b200 import _lib
+
+    lib = _lib.load()
+    B, H, G, D, n = 3, 2, 4, 128, 9000
+    P = B * H
+    x, y, q = _rows((B, H, n, D), "bf16", 180, False), _rows((B, H, n, D), "bf16", 181, False), _rows((B, H * G, D), "bf16", 182, False)
+    lens = torch.tensor([9000, 0, 700], dtype=torch.int32, device="cuda")
+    st = int(torch.cuda.current_stream().cuda_stream)
+    bufs = [torch.zeros((P, n, d), dtype=t, device="cuda") for _ in range(2) for d, t in ((D // 2, torch.uint8), (D // 32, torch.bfloat16))]
+    dx, dy, dq = x.cuda(), y.cuda(), q.cuda()
+    _lib.check(lib.dc_q4_write_rows(dx.data_ptr(), dy.data_ptr(), H * n * D, n * D, D, P, H, n, D, 0, *(t.data_ptr() for t in bufs), n, 0, st))
+    out = torch.full_like(dq, 7.0)
+    acc, ml = torch.full((B, H * G, D), 7.0, device="cuda"), torch.full((B, H * G, 2), 7.0, device="cuda")
+    scratch = torch.full((int(lib.dc_q4_attend_scratch_bytes(P, G, D)) // 4,), math.nan, device="cuda")
+    dst = (None, None, acc.data_ptr(), ml.data_ptr()) if partials else (out.data_ptr(), None, None, None)
+    _lib.check(lib.dc_q4_attend(*(t.data_ptr() for t in bufs), n, n, P, H, G, D, 0, dq.data_ptr(), None, 0, -1, 0, lens.data_ptr(),
+                                None, None, None, None, 0, 0, 0, 0.0, *dst, scratch.data_ptr(), st))
+    if partials:
+        _lib.check(lib.dc_lse_combine(acc.data_ptr(), acc.numel(), ml.data_ptr(), ml.numel(), 1, B * H * G, D, 0, out.data_ptr(), None, st))
+    torch.cuda.synchronize()
+    for b in range(B):
+        m = int(lens[b])
+        for h in range(H):
+            got = out[b, h * G:(h + 1) * G].cpu()[None]
+            if m == 0:
+                assert (got == 0).all()
+                continue
+            want, _, tol, _ = q4_util.attend(q[b, h * G:(h + 1) * G][None], q4_util.stored(x[b, h, :m])[None],
+                                             q4_util.stored(y[b, h, :m])[None], torch.ones(1, m, dtype=torch.bool), D ** -0.5)
+            q4_util.assert_close(got, want, tol, f"out {b},{h}")
+
+
+@pytest.mark.parametrize("B,H,G,D,n", [(1, 2, 4, 128, 20001), (1, 1, 8, 256, 9000), (1, 3, 1, 64, 12345), (2, 1, 12, 128, 7000)])
+def test_attend_many_partials(B, H, G, D, n):
+    """Few problems with many rows: more CTAs than a cluster holds, merged by a second kernel."""
+    _attend_case(B, H, G, D, n, "bf16", 190, res=130, new=True)
+    _attend_case(B, H, G, D, n, "fp16", 191)
+    _attend_case(B, H, G, D, n, "bf16", 192, lens=torch.tensor([n - 3, 100][:B], dtype=torch.int32), res=2)
+    gen = torch.Generator().manual_seed(4)
+    ids = torch.stack([torch.randperm(n, generator=gen)[:6500] for _ in range(B * H)]).reshape(B, H, 6500).to(torch.int32)
+    _attend_case(B, H, G, D, n, "fp16", 193, ids=ids, new=True)
+
+
 def test_refusals():
     from diffcache_b200 import DiffCacheError
 
