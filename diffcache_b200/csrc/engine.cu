@@ -433,6 +433,7 @@ int q4_rows_in(dc_engine* e, const void* keys, const void* vals, int64_t n, int6
         return q4_write_rows(keys, vals, stride_b, stride_h, stride_s, e->n_prob, e->kv_heads, n, e->head_dim, e->dtype,
                              e->st, row0, e->len, len_mode, s);
     const int64_t D = e->head_dim, piece = std::min<int64_t>(n, 65536);
+    if (n == 1) stride_s = D;   // never used, and may be anything
     const size_t es = sizeof(uint16_t);
     uint16_t* stage = nullptr;
     int rc = DC_OK;
@@ -777,8 +778,9 @@ int dc_get_keys(dc_engine* e, float* out) {
             Q4Store st = e->st;
             st.k.codes += static_cast<int64_t>(p0) * st.prob_rows * q4_code_bytes(e->head_dim);
             st.k.scales += static_cast<int64_t>(p0) * st.prob_rows * (e->head_dim / kQ4Group);
-            q4_read_rows(st, ctx, nullptr, np, e->head_dim, e->dtype, 0, nullptr, 0, ctx, dst, nullptr, true, nullptr);
-            return cudaGetLastError();
+            const int rc = q4_read_rows(st, ctx, nullptr, np, e->head_dim, e->dtype, 0, nullptr, 0, ctx, dst, nullptr, true, nullptr);
+            const cudaError_t last = cudaGetLastError();
+            return rc != DC_OK && last == cudaSuccess ? cudaErrorUnknown : last;
         }
         const uint16_t* src = e->k + static_cast<int64_t>(p0) * e->prob_stride;
         if (e->dtype == DC_BF16) keys_to_f32_kernel<DC_BF16><<<grid, 256>>>(src, e->prob_stride, ctx, e->head_dim, dst);
@@ -889,6 +891,7 @@ int dc_write_rows(dc_engine* e, const void* keys, const void* vals, int64_t row0
                    ((reinterpret_cast<uintptr_t>(keys) | reinterpret_cast<uintptr_t>(vals)) & 15) == 0,
                "dc_write_rows: pointers must be 16-byte aligned and strides non-negative multiples of 8 elements");
     cudaStream_t s = as_stream(stream);
+    if (n == 1) stride_s = e->head_dim;   // never used, and may be anything
     int rc = DC_OK;
     if (e->q4) {
         rc = q4_rows_in(e, keys, vals, n, row0, stride_b, stride_h, stride_s, kLenMax, s);

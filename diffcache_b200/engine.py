@@ -119,6 +119,12 @@ def _device_stream(device: int) -> int:
     return int(_raw_stream_getter()(device))
 
 
+def _alike(x, y) -> bool:
+    """Two tensors of one shape, type, device and layout: what holds for one holds for the other."""
+    return (type(x) is type(y) and _is_torch(x) and x.shape == y.shape and x.dtype is y.dtype and
+            x.get_device() == y.get_device() and x.stride() == y.stride())
+
+
 def _row_strides(x, what: str):
     """Element strides of the (batch, head, row) axes; 0 for an axis of size 1, whose stride is never used."""
     if isinstance(x, np.ndarray):
@@ -314,10 +320,11 @@ class DiffCacheGPU:
         ``keys``/``vals`` ``(bsz, kv_head_num, n, head_dim)`` as in :meth:`prefill`.  ``row0`` may be at most
         ``ctx_len``; the store then holds ``max(ctx_len, row0 + n)`` rows."""
         n = self._rows(keys, None, "keys")
-        self._rows(vals, n, "vals")
         sb, sh, ss = _row_strides(keys, "keys")
-        if _row_strides(vals, "vals") != (sb, sh, ss):
-            raise ValueError("keys and vals must share one stride pattern")
+        if not _alike(keys, vals):
+            self._rows(vals, n, "vals")
+            if _row_strides(vals, "vals") != (sb, sh, ss):
+                raise ValueError("keys and vals must share one stride pattern")
         _lib.check(self._lib.dc_write_rows(self._h, _ptr(keys), _ptr(vals), int(row0), n, sb, sh, ss, self._stream(stream)))
 
     def read_rows(self, out_keys, out_vals, row0: int = 0, ids=None, stream=None) -> None:
@@ -326,7 +333,7 @@ class DiffCacheGPU:
         kv_head_num, n)`` int32.  Rows that are not stored (negative ids, positions beyond ``ctx_len``) are zeros."""
         n = None
         for x, what in ((out_keys, "out_keys"), (out_vals, "out_vals")):
-            if x is not None:
+            if x is not None and not (n is not None and _alike(out_keys, x)):
                 self._on_device(x, what)
                 n = self._rows(x, n, what)
                 _require_contiguous(x, what)
@@ -358,7 +365,7 @@ class DiffCacheGPU:
         self._heads(q, self.q_head_num, "q")
         self._heads(out, self.q_head_num, "out")
         _require_contiguous(out, "out")
-        qsb = 0 if q.is_contiguous() else self._batch_stride(q, self.q_head_num, "q")
+        qsb = 0 if q.is_contiguous() else self._slice_stride(q, self.q_head_num, "q")
         n_ids, ids_ptr, lens_ptr, lse_ptr, kn_ptr, vn_ptr, nsb, rk_ptr, rv_ptr, sb, sh = -1, None, None, None, None, None, 0, None, None, 0, 0
         if ids is not None:
             if lens is not None:
@@ -382,32 +389,40 @@ class DiffCacheGPU:
             self._heads(k_new, self.kv_head_num, "k_new")
             self._heads(v_new, self.kv_head_num, "v_new")
             if not (k_new.is_contiguous() and v_new.is_contiguous()):
-                nsb = self._batch_stride(k_new, self.kv_head_num, "k_new")
-                if self._batch_stride(v_new, self.kv_head_num, "v_new") != nsb:
+                nsb = self._slice_stride(k_new, self.kv_head_num, "k_new")
+                if self._slice_stride(v_new, self.kv_head_num, "v_new") != nsb:
                     raise ValueError("k_new and v_new must have the same batch stride")
             kn_ptr, vn_ptr = k_new.data_ptr(), v_new.data_ptr()
             need += 1
         if res_k is not None:
             self._on_device(res_k, "res_k")
-            self._on_device(res_v, "res_v")
             rows = self._rows(res_k, None, "res_k")
-            self._rows(res_v, rows, "res_v")
+            sb, sh, ss = _row_strides(res_k, "res_k")
+            if not _alike(res_k, res_v):
+                self._on_device(res_v, "res_v")
+                self._rows(res_v, rows, "res_v")
+                if (sb, sh, ss) != _row_strides(res_v, "res_v"):
+                    raise ValueError("res_k/res_v must share strides with contiguous rows of head_dim")
             if rows < need:
                 raise ValueError(f"res_k/res_v hold {rows} rows, the call needs {need}")
-            sb, sh, ss = _row_strides(res_k, "res_k")
-            if (sb, sh, ss) != _row_strides(res_v, "res_v") or ss not in (0, self.head_dim):
+            if ss not in (0, self.head_dim):
                 raise ValueError("res_k/res_v must share strides with contiguous rows of head_dim")
             rk_ptr, rv_ptr = res_k.data_ptr(), res_v.data_ptr()
         elif res_len:
             raise ValueError("res_len > 0 needs res_k and res_v")
         _lib.check(self._lib.dc_attend_rows(self._h, q.data_ptr(), qsb, ids_ptr, n_ids, lens_ptr, kn_ptr, vn_ptr, nsb, rk_ptr, rv_ptr,
-                                            sb, sh, int(res_len), scale, out.data_ptr(), lse_ptr, self._stream(stream)))
+                                            sb, sh, int(res_len), float(scale), out.data_ptr(), lse_ptr, self._stream(stream)))
 
     # Argument checks of the calls above.  They are the larger part of a small call's time, so each looks at an
     # attribute once.
     def _stream(self, stream) -> int:
         """The given stream, else the current stream of this engine's device."""
         return _device_stream(self.device) if stream is None else int(stream)
+
+    def _slice_stride(self, x, heads: int, what: str) -> int:
+        if self.bsz > 1 and x.stride(0) == 0:   # 0 means dense to the engine
+            raise ValueError(f"{what} must not be expanded over the batch")
+        return self._batch_stride(x, heads, what)
 
     def _on_device(self, x, what: str) -> None:
         if not _is_torch(x):

@@ -729,6 +729,96 @@ def test_attend_many_partials(B, H, G, D, n):
     _attend_case(B, H, G, D, n, "fp16", 193, ids=ids, new=True)
 
 
+def test_adaptive_budget_on_a_4_bit_store():
+    """The k-check works on the 4-bit scan's keys, and attention stops at its budget."""
+    B, H, G, D, n, topk = 1, 3, 4, 128, 2000, 400
+    x, y, q = _rows((B, H, n, D), "bf16", 200, False), _rows((B, H, n, D), "bf16", 201, False), _rows((B, H * G, D), "bf16", 202, False)
+    q[:, :G] += x[0, 0, 5] * 0.5          # a head group whose mass sits on few rows
+    eng = _engine(B, H, G, D, n, adaptive_budget=True, k_check_seq=[25, 50, 100, 200], attn_mass_threshold=0.5)
+    eng.prefill(x.cuda(), y.cuda())
+    out, idx = torch.empty_like(q, device="cuda"), torch.empty(B, H, topk, dtype=torch.int32, device="cuda")
+    eng.decode_attend(q.cuda(), out, topk, out_idx=idx)
+    budget = eng.last_budget()
+    assert budget.min() >= 1 and budget.max() <= topk
+    ks, vs = q4_util.stored(x), q4_util.stored(y)
+    for h in range(H):
+        pick = idx[0, h, :int(budget[0, h])].cpu().long()
+        want, _, tol, _ = q4_util.attend(q[0, h * G:(h + 1) * G][None], ks[0, h][pick][None], vs[0, h][pick][None],
+                                         torch.ones(1, len(pick), dtype=torch.bool), D ** -0.5)
+        q4_util.assert_close(out[0, h * G:(h + 1) * G].cpu()[None], want, tol, f"head {h}")
+
+
+def test_offsets_beyond_32_bits():
+    """Rows more than 4 GB into a problem's codes: written, read back, scored and attended."""
+    from diffcache_b200 import _lib
+
+    lib = _lib.load()
+    G, D, rows, n = 4, 128, 68_000_000, 300
+    if torch.cuda.mem_get_info()[0] < 16 << 30:
+        pytest.skip("needs 12 GB of device memory")
+    first = rows - n
+    x, y, q = _rows((1, 1, n, D), "bf16", 210), _rows((1, 1, n, D), "bf16", 211), _rows((1, G, D), "bf16", 212, False)
+    dx, dy, dq = x.cuda(), y.cuda(), q.cuda()
+    st = int(torch.cuda.current_stream().cuda_stream)
+    bufs = [torch.full((1, rows, d), fill, dtype=t, device="cuda") for _ in range(2)
+            for d, t, fill in ((D // 2, torch.uint8, 0x88), (D // 32, torch.bfloat16, 0.0))]
+    _lib.check(lib.dc_q4_write_rows(dx.data_ptr(), dy.data_ptr(), 0, 0, D, 1, 1, n, D, 0, *(t.data_ptr() for t in bufs), rows, first, st))
+    back = torch.empty_like(dx)
+    _lib.check(lib.dc_q4_read_rows(bufs[2].data_ptr(), bufs[3].data_ptr(), rows, rows, 1, D, 0, first, None, 0, n, back.data_ptr(), st))
+    assert bit_rows(back, q4_util.stored(y).to(y.dtype))
+    mean = dq.float().mean(1).to(dq.dtype).contiguous()
+    bits = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    _lib.check(lib.dc_q4_score_scan(bufs[0].data_ptr(), bufs[1].data_ptr(), rows, 1, rows, D, 0, mean.data_ptr(), 0, 1, bits.data_ptr(), rows, None, st))
+    dist, tol = q4_util.scan(q4_util.stored(x).reshape(1, n, D), mean.cpu())
+    q4_util.assert_close(bits[first:].cpu().view(torch.float32)[None], dist, tol, "dist")
+    assert (bits[:first].view(torch.float32) == 65536.0).all()
+    ids = torch.arange(first, rows, dtype=torch.int32, device="cuda")
+    out = torch.empty_like(dq)
+    scratch = torch.empty(int(lib.dc_q4_attend_scratch_bytes(1, G, D)), dtype=torch.uint8, device="cuda")
+    _lib.check(lib.dc_q4_attend(*(t.data_ptr() for t in bufs), rows, rows, 1, 1, G, D, 0, dq.data_ptr(), ids.data_ptr(), n, n, 0, None,
+                                None, None, None, None, 0, 0, 0, 0.0, out.data_ptr(), None, None, None, scratch.data_ptr(), st))
+    want, _, wtol, _ = q4_util.attend(q, q4_util.stored(x)[0], q4_util.stored(y)[0], torch.ones(1, n, dtype=torch.bool), D ** -0.5)
+    q4_util.assert_close(out.cpu(), want, wtol, "ids")
+    # every row: the zero rows in front score 0 and weigh in with values of 0
+    _lib.check(lib.dc_q4_attend(*(t.data_ptr() for t in bufs), rows, rows, 1, 1, G, D, 0, dq.data_ptr(), None, 0, -1, 0, None,
+                                None, None, None, None, 0, 0, 0, 0.0, out.data_ptr(), None, None, None, scratch.data_ptr(), st))
+    x64 = torch.matmul(q[0].double(), q4_util.stored(x)[0, 0].T) * D ** -0.5
+    e = torch.exp(x64)
+    total = e.sum(-1, keepdim=True) + first
+    ref = torch.matmul(e, q4_util.stored(y)[0, 0]) / total
+    spread = torch.matmul(e, q4_util.stored(y)[0, 0].abs()) / total
+    # a warp adds its share of the rows 16 at a time, each step off by at most 2^-23 of the running sum; at least 255 CTAs of
+    # four warps share the rows
+    rel = rows / (4 * 255 * 16) * 2.0 ** -23 + 2.0 ** -12
+    q4_util.assert_close(out.cpu()[0], ref, rel * spread + 2.0 ** -8 * ref.abs() + 2.0 ** -30, "all")
+
+
+def test_inputs_that_would_be_read_wrongly_are_refused():
+    B, H, G, D, n = 2, 2, 2, 64, 10
+    eng = _engine(B, H, G, D, 16)
+    x = _rows((B, H, n, D), "bf16", 220)
+    eng.prefill(x.cuda(), x.cuda())
+    q = _rows((1, H * G, D), "bf16", 221, False).cuda()
+    out = torch.empty(B, H * G, D, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="expanded"):
+        eng.attend_rows(q.expand(B, H * G, D), out)
+    kn = q[:, :H].contiguous()
+    with pytest.raises(ValueError, match="expanded"):
+        eng.attend_rows(q.repeat(B, 1, 1), out, k_new=kn.expand(B, H, D), v_new=kn.expand(B, H, D))
+    for shape in ((B, H, 1, D),):          # a host row whose row stride means nothing
+        row = torch.zeros(shape, dtype=torch.bfloat16)
+        eng.write_rows(n, row, row)
+    assert eng.ctx_len == n + 1
+    from diffcache_b200 import DiffCacheGPU
+
+    wide = DiffCacheGPU(B, H * G, H, D, max_ctx_len=16)
+    wide.write_rows(0, row, row)
+    wide.write_rows(1, util.u16(x), util.u16(x))
+    back = torch.empty(B, H, n, D, dtype=torch.bfloat16, device="cuda")
+    wide.read_rows(back, None, row0=1)
+    assert torch.equal(back.cpu(), x)
+
+
 def test_refusals():
     from diffcache_b200 import DiffCacheError
 
