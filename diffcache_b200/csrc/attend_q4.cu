@@ -1,6 +1,11 @@
 // Attention over a store held in 4 bits (format: q4.cuh), the resident 16-bit rows and the new token, with split-K
 // and log-sum-exp merge: the 4-bit counterpart of attend.cu (flash_attn_with_kvcache over the gathered buffer,
 // src/diffcache/base.py:134-142), over the rows of an id list or over every stored row of a sequence.
+//
+// Bound, at head_dim 128 and four query heads: 144 bytes a row against 425 instructions per 16 rows, most of them turning
+// nibbles into fragment values.  64 problems x 32768 consecutive rows: 84 us = 3.6 TB/s of codes and scales, 2.7 instructions
+// per clock, integer pipe 60 % (simple kernel: 3400 us; operands loaded to registers without the ring: 116; keys as the
+// columns of B instead of the rows of A: 110).  16384 random rows each: 65 us, 4.7 TB/s of DRAM traffic, twice the bytes used.
 #include <cooperative_groups.h>
 
 #include <algorithm>
