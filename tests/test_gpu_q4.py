@@ -549,6 +549,121 @@ def test_sharded_halves_equal_one_engine():
     q4_util.assert_close(want.cpu().reshape(H, G, D), ref, tol, "whole")
 
 
+@pytest.mark.parametrize("n,topk,world", [(1500, 64, 2), (7, 16, 3)])
+def test_sequence_sharded_step_over_peer_stores(n, topk, world):
+    """The sequence-sharded step on 4-bit engines with both exchanges done by the step's kernels, all ranks emulated on this
+    GPU phase by phase (the small case leaves ranks with a few rows and pads)."""
+    import ctypes
+
+    from diffcache_b200 import sharded
+
+    B, H, G, D, res = 1, 2, 4, 128, 9
+    x, y, q = _rows((B, H, n, D), "bf16", 230), _rows((B, H, n, D), "bf16", 231), _rows((B, H * G, D), "bf16", 232, False)
+    rk, rv = _rows((B, H, res + 2, D), "bf16", 233, False), _rows((B, H, res + 2, D), "bf16", 234, False)
+    kn, vn = _rows((B, H, D), "bf16", 235, False), _rows((B, H, D), "bf16", 236, False)
+    engines, backends = [], []
+    for r, (start, length) in enumerate(sharded.shard_rows(n, world)):
+        e = _engine(B, H, G, D, max(length, 1))
+        if length:
+            e.prefill(x[:, :, start:start + length].contiguous().cuda(), y[:, :, start:start + length].contiguous().cuda())
+        last = r == world - 1
+        engines.append(e)
+        backends.append(sharded.GpuShardBackend(e, start, rk.cuda() if last else None, rv.cuda() if last else None, res if last else 0,
+                                                kn.cuda() if last else None, vn.cuda() if last else None))
+    need = (ctypes.c_int64 * 2)()
+    assert backends[0].lib.dc_sharded_slot_bytes(engines[0]._h, topk, need) == 0
+    xs = sharded.PeerExchange.in_process([int(need[0]), int(need[1])], [torch.cuda.current_device()] * world)
+    qd = q.cuda()
+    for _ in range(2):
+        for phase in range(3):
+            outs = [b.peer_phase(phase, qd, topk, z) for b, z in zip(backends, xs)]
+        torch.cuda.synchronize()
+    assert all(torch.equal(o, outs[0]) for o in outs)
+    for z in xs:
+        z.check()
+        z.close()
+    whole = _engine(B, H, G, D, n)
+    whole.prefill(x.cuda(), y.cuda())
+    k = min(topk, n)
+    one, idx = torch.empty_like(qd), torch.empty(B, H, k, dtype=torch.int32, device="cuda")
+    whole.decode_attend(qd, one, topk, res_k=rk.cuda(), res_v=rv.cuda(), res_len=res, k_new=kn.cuda(), v_new=vn.cuda(), out_idx=idx)
+    ks, vs = q4_util.stored(x), q4_util.stored(y)
+    for h in range(H):
+        pick = idx[0, h].cpu().long()
+        kk = torch.cat([ks[0, h][pick], rk[0, h, :res].double(), kn[0, h].double()[None]])
+        vv = torch.cat([vs[0, h][pick], rv[0, h, :res].double(), vn[0, h].double()[None]])
+        want, _, tol, _ = q4_util.attend(q[0, h * G:(h + 1) * G][None], kk[None], vv[None], torch.ones(1, len(kk), dtype=torch.bool),
+                                         D ** -0.5)
+        q4_util.assert_close(outs[0].reshape(H, G, D)[h].cpu()[None], want, tol, f"sharded {h}")
+        q4_util.assert_close(one[0, h * G:(h + 1) * G].cpu()[None], want, tol, f"whole {h}")
+
+
+def test_kv_cache_manager_prefill_cache_round_trip(tmp_path):
+    from diffcache_b200 import DiffCache
+
+    L, B, H, G, D, S = 2, 2, 2, 4, 64, 300
+    kw = dict(num_layers=L, batch_size=B, max_length=S + 32, num_kv_heads=H, num_q_heads=H * G, head_dim=D, retrieval_budget=64,
+              kvbuf_prefix_len=16, kvbuf_suffix_len=24, kvbuf_suffix_maxlen=48, store_bits=4)
+    a = DiffCache(**kw)
+    for l in range(L):
+        a.prefill_update_kv_cache(_rows((B, S, H, D), "bf16", 240 + l, False).cuda(), _rows((B, S, H, D), "bf16", 250 + l, False).cuda(), l)
+    (tmp_path / "cache").mkdir()
+    a.save_prefill_cache(str(tmp_path / "cache"))
+    b = DiffCache(**kw)
+    b.load_prefill_cache(torch.zeros((B, S), dtype=torch.long), str(tmp_path / "cache"))
+    for l in range(L):
+        q, kn, vn = (_rows((B, 1, h * D), "bf16", 260 + h, False).cuda() for h in (H * G, H, H))
+        ia, ib = torch.zeros((B, H, 64), dtype=torch.int32, device="cuda"), torch.zeros((B, H, 64), dtype=torch.int32, device="cuda")
+        oa = a.decode_attention(l, q, kn.view(B, 1, H, D), vn.view(B, 1, H, D), out_idx=ia)
+        ob = b.decode_attention(l, q, kn.view(B, 1, H, D), vn.view(B, 1, H, D), out_idx=ib)
+        assert torch.equal(ia, ib) and torch.equal(oa, ob)
+    # the reference's three-call shape: the retrieved rows arrive in the element type
+    c = DiffCache(**kw)
+    k, v = _rows((B, S, H, D), "bf16", 240, False), _rows((B, S, H, D), "bf16", 250, False)
+    c.prefill_update_kv_cache(k.cuda(), v.cuda(), 0)
+    c.decode_pre_query_operation(_rows((B, 1, H * G * D), "bf16", 270, False).cuda())
+    c.decode_query_kvcache(0)
+    c.decode_post_query_operation(0)
+    got = c.get_kvcache(0)[0][:, :64].permute(0, 2, 1, 3).cpu()
+    mid = (q4_util.stored(k[:, 16:S - 24].permute(0, 2, 1, 3)) + 0.0).to(torch.bfloat16)   # + 0.0: a zero without sign
+    for bb in range(B):
+        for h in range(H):
+            rows = {tuple(r.tolist()) for r in mid[bb, h].view(torch.int16)}
+            assert all(tuple(r.tolist()) in rows for r in got[bb, h].view(torch.int16))
+
+
+def test_attention_stack_on_4_bit_stores():
+    from diffcache_b200.stack import AttentionStack
+
+    B, HQ, H, D, n, topk, sink, win = 2, 8, 2, 128, 700, 96, 16, 32
+    st = AttentionStack(2, 256, B, HQ, H, D, n, topk, sink, win, store_bits=4)
+    probe = {}
+    x = torch.randn(B, 256, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    out = st.step(x, probe=probe)
+    assert torch.isfinite(out).all() and all(e.store_bits == 4 for e in st.engines)
+    eng, n_r = st.engines[0], n - sink - win
+    idx = torch.empty(B, H, topk, dtype=torch.int32, device="cuda")
+    again = torch.empty_like(probe["attn"])
+    eng.decode_attend(probe["q"].contiguous(), again, topk, res_k=st.res_k[0], res_v=st.res_v[0], res_len=st.res_rows,
+                      k_new=probe["k_new"].contiguous(), v_new=probe["v_new"].contiguous(), out_idx=idx)
+    assert torch.equal(again, probe["attn"])
+    codes = torch.empty(B, H, n_r, D, dtype=torch.bfloat16, device="cuda"), torch.empty(B, H, n_r, D, dtype=torch.bfloat16, device="cuda")
+    eng.read_rows(*codes)        # the stored rows rounded to the element type: within half a step of what is attended
+    G = HQ // H
+    for b in range(B):
+        for h in range(H):
+            pick = idx[b, h].cpu().long()
+            kk = torch.cat([codes[0][b, h].cpu()[pick], st.res_k[0][b, h, :st.res_rows].cpu(), probe["k_new"][b, h].cpu()[None]]).double()
+            vv = torch.cat([codes[1][b, h].cpu()[pick], st.res_v[0][b, h, :st.res_rows].cpu(), probe["v_new"][b, h].cpu()[None]]).double()
+            q = probe["q"][b, h * G:(h + 1) * G].cpu()
+            want, _, tol, _ = q4_util.attend(q[None], kk[None], vv[None], torch.ones(1, len(kk), dtype=torch.bool), D ** -0.5)
+            # every key element off by half a step moves a logit by that part of the magnitudes it sums; values likewise
+            mag = (q.double().abs() @ kk.abs().T).amax() * D ** -0.5
+            slack = (2 * 2.0 ** -8 * mag + 2.0 ** -8) * vv.abs().amax()
+            q4_util.assert_close(probe["attn"][b, h * G:(h + 1) * G].cpu()[None], want, tol + slack, "attn")
+    st.close()
+
+
 def test_decode_loop_with_ring_and_spill_from_one_graph():
     """A KV-cache manager on 4-bit stores: captured decode steps past the full window; spilled tokens land in the store."""
     from diffcache_b200 import DiffCache
