@@ -28,6 +28,7 @@ constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kHeads = 8;            // query heads of one kv head handled by one CTA (columns of the second product)
 constexpr int kTile = 16;            // rows a warp takes at a time
+constexpr int kMaxCluster = 8;        // CTAs of a problem that finish its output together (the portable cluster size)
 constexpr float kLog2e = 1.4426950408889634f;
 __host__ __device__ constexpr int ctas_per_sm(int head_dim) { return head_dim <= 128 ? 4 : 2; }
 
@@ -343,12 +344,16 @@ q4_attend_kernel(const Args a) {
         id[0] = id[R::STAGES - 1];
         __syncthreads();                               // the query is in shared memory
         // query fragments, normalised to [2^14, 2^15) by a power of two
-        float top = 0.0f;
-        for (int d = t; d < D; d += 4) top = fmaxf(top, fabsf(elem_to_float<DT>(qrow[d])));
-        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+        uint32_t top = 0;                              // magnitude bits order like magnitudes
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) {
+            const uint4 w = *reinterpret_cast<const uint4*>(qrow + 32 * i + 8 * t);
+            top = __vmaxu2(top, __vmaxu2(__vmaxu2(w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu), __vmaxu2(w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu)));
+        }
+        top = __vmaxu2(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+        top = __vmaxu2(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
         float down, up_g;
-        q4_normalise(top, down, up_g);
+        q4_normalise(elem_to_float<DT>(static_cast<uint16_t>(max(top & 0xFFFFu, top >> 16))), down, up_g);
         up_g *= a.scale_log2;
         const float up[2] = {__shfl_sync(0xFFFFFFFFu, up_g, 8 * t), __shfl_sync(0xFFFFFFFFu, up_g, 8 * t + 4)};   // heads 2t, 2t + 1
         uint32_t qa[NT][2];
@@ -359,10 +364,9 @@ q4_attend_kernel(const Args a) {
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
                     const int d = 16 * (4 * w + 2 * gp) + 2 * (2 * t + c);   // a tile's element; + 16 is the group's other tile
-#pragma unroll
-                    for (int e = 0; e < 2; e++)
-                        qa[4 * w + 2 * gp + c][e] = pack2<false>(elem_to_float<DT>(qrow[d + e]) * down,
-                                                                 elem_to_float<DT>(qrow[d + 16 + e]) * down);
+                    const uint32_t w0 = *reinterpret_cast<const uint32_t*>(qrow + d), w1 = *reinterpret_cast<const uint32_t*>(qrow + d + 16);
+                    qa[4 * w + 2 * gp + c][0] = pack2<false>(low_elem<DT>(w0) * down, low_elem<DT>(w1) * down);
+                    qa[4 * w + 2 * gp + c][1] = pack2<false>(high_elem<DT>(w0) * down, high_elem<DT>(w1) * down);
                 }
 
         const CodeConst cc(static_cast<uint32_t>(a.kv_heads) >> 31);
@@ -606,17 +610,28 @@ q4_attend_kernel(const Args a) {
     const int n_part = a.n_split / a.cluster, part = split / a.cluster;
     for (int e = (split % a.cluster) * kThreads + tid; e < n_heads * D; e += a.cluster * kThreads) {
         const int head = e / D, d = e % D;
-        float mx = -INFINITY;
-        for (int r = 0; r < a.cluster; r++) mx = fmaxf(mx, cluster.map_shared_rank(&s_sum[0][0], r)[2 * head]);
+        // everything the other CTAs hold is requested before any of it is used; a CTA without rows has zeros
+        float mr[kMaxCluster], lr[kMaxCluster], ar[kMaxCluster];
+#pragma unroll
+        for (int r = 0; r < kMaxCluster; r++) {
+            if (r < a.cluster) {
+                const float* ml = cluster.map_shared_rank(&s_sum[0][0], r);
+                mr[r] = ml[2 * head];
+                lr[r] = ml[2 * head + 1];
+                ar[r] = cluster.map_shared_rank(&s_o[0][0][0], r)[head * (D + 4) + d];
+            } else {
+                mr[r] = -INFINITY; lr[r] = 0.0f; ar[r] = 0.0f;
+            }
+        }
+        float mx = mr[0];
+#pragma unroll
+        for (int r = 1; r < kMaxCluster; r++) mx = fmaxf(mx, mr[r]);
         float acc = 0.0f, sum = 0.0f;
-        for (int r = 0; r < a.cluster; r++) {
-            const float* ml = cluster.map_shared_rank(&s_sum[0][0], r);
-            const float mr = ml[2 * head], lr = ml[2 * head + 1];
-            const float ar = cluster.map_shared_rank(&s_o[0][0][0], r)[head * (D + 4) + d];
-            if (mr == -INFINITY && lr == 0.0f) continue;   // a CTA without rows
-            const float f = exp2f(mr - mx);
-            acc += ar * f;
-            sum += lr * f;
+#pragma unroll
+        for (int r = 0; r < kMaxCluster; r++) {
+            const float f = mr[r] == -INFINITY && lr[r] == 0.0f ? 0.0f : exp2f(mr[r] - mx);
+            acc = fmaf(ar[r], f, acc);
+            sum = fmaf(lr[r], f, sum);
         }
         const int64_t row = prob * a.group + g0 + head;
         if (a.out != nullptr) {
@@ -691,7 +706,6 @@ q4_merge_kernel(const float* __restrict__ part_acc, const float* __restrict__ pa
             out_lse[row] = some ? (mx + log2f(sum)) * 0.6931471805599453f : -INFINITY;
     }
 }
-constexpr int kMaxCluster = 8;   // the portable size
 
 template <int DT, int D, bool FEW, bool IDS>
 int launch_one(const Args& a, dim3 grid, cudaStream_t stream) {
