@@ -2,10 +2,10 @@
 // and log-sum-exp merge: the 4-bit counterpart of attend.cu (flash_attn_with_kvcache over the gathered buffer,
 // src/diffcache/base.py:134-142), over the rows of an id list or over every stored row of a sequence.
 //
-// Bound, at head_dim 128 and four query heads: 144 bytes a row against 425 instructions per 16 rows, most of them turning
-// nibbles into fragment values.  64 problems x 32768 consecutive rows: 84 us = 3.6 TB/s of codes and scales, 2.7 instructions
-// per clock, integer pipe 60 % (simple kernel: 3400 us; operands loaded to registers without the ring: 116; keys as the
-// columns of B instead of the rows of A: 110).  16384 random rows each: 65 us, 4.7 TB/s of DRAM traffic, twice the bytes used.
+// Bound, at head_dim 128 and four query heads: 144 bytes a row against 407 instructions per 16 rows, most of them turning
+// nibbles into fragment values.  64 problems x 32768 consecutive rows: 79 us = 3.8 TB/s of codes and scales, 2.7 instructions
+// per clock (operands loaded to registers without the ring: 116; keys as the columns of B instead of the rows of A: 110;
+// weights scaled and split in fp32: 83).  16384 random rows each: 65 us, 4.7 TB/s of DRAM traffic, twice the bytes used.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -128,6 +128,20 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t keep_lo, u
         hi = FEW && keep_lo != 0x4444u ? rest : r;
     }
 }
+// Weights times bf16 scales, again as a bf16 value and its remainder, in packed bf16: with the weight as h + x,
+//   hi = round(h s),  lo = round(x s + (h s - hi)),
+// where h s - hi is exact (16 significant bits less the 8 kept).  hi + lo is the product to 2^-15: the remainder of a
+// weight is kept to 2^-16 of it, and lo, at most 2^-7 of the product, is rounded once.  With few heads the lanes that hold
+// the value pass h = 0 and the value as x, so that lo is round(h s) there and the remainder in the others.
+template <bool FEW>
+__device__ __forceinline__ void scale_pair(uint32_t h, uint32_t x, uint32_t s, uint32_t& hi, uint32_t& lo) {
+    uint32_t v, e;
+    asm("mul.rn.bf16x2 %0, %1, %2;\n" : "=r"(v) : "r"(h), "r"(s));
+    asm("{\n .reg .b32 n;\n neg.bf16x2 n, %3;\n fma.rn.bf16x2 %0, %1, %2, n;\n}\n" : "=r"(e) : "r"(h), "r"(s), "r"(v));
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;\n" : "=r"(lo) : "r"(x), "r"(s), "r"(e));
+    hi = FEW ? lo : v;
+}
+
 __device__ __forceinline__ float exp2_fast(float x) {   // 2^x to 2 ulp, 0 below 2^-126 and for -inf
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(x));
@@ -184,8 +198,8 @@ __device__ __forceinline__ void transpose_weights(const float (&x)[4], float (&y
 // codes enter as small integers (fp16, exact), so a group's partial product is exact up to fp32 accumulation and its scale
 // is applied once, in fp32.  The query of a head is normalised by a power of two so that a bf16 query is exact in fp16 too.
 // O^T = V^T P^T: the value codes are A (16 elements of a tile x 16 rows, bf16 integers), the weights are B; a value's scale
-// depends on (row, group) only, so it multiplies the weight, which then enters as a bf16 value and its remainder
-// (16 bits).  With at most four heads value and remainder are two column groups of ONE MMA (columns h and h + 4),
+// depends on (row, group) only, so it multiplies the weight, which enters as a bf16 value and its remainder
+// (scale_pair for bf16 scales, split_pair for the 11 bits of fp16 ones).  With at most four heads value and remainder are two column groups of ONE MMA (columns h and h + 4),
 // otherwise two MMAs.  The rows of a tile are numbered so that a lane's rows in both fragments are 4t .. 4t + 3.
 // Every warp streams its tiles through a ring of its own in shared memory, three tiles ahead of the arithmetic; the stored
 // order of the codes makes each lane's share of a row one load.  Warps are independent until the end.
@@ -422,6 +436,15 @@ q4_attend_kernel(const Args a) {
             softmax_step<NT>(sc, m, l, o);
             float wt[4];
             transpose_weights(sc, wt, g, t);
+            uint32_t ph[2], px[2];                     // the weights as value and remainder (scale_pair)
+            if (BF16)
+#pragma unroll
+                for (int blk = 0; blk < 2; blk++) {
+                    const uint32_t r = pack2<true>(wt[2 * blk], wt[2 * blk + 1]);
+                    const uint32_t rest = pack2<true>(wt[2 * blk] - low_elem<DC_BF16>(r), wt[2 * blk + 1] - high_elem<DC_BF16>(r));
+                    ph[blk] = FEW && g < 4 ? 0u : r;
+                    px[blk] = FEW && g < 4 ? r : rest;
+                }
             constexpr int WV = D == 64 ? 1 : 2;        // words of a row's values and scales read at a time
             uint32_t vw[4][WV], vs[4][WV];
 #pragma unroll
@@ -438,10 +461,15 @@ q4_attend_kernel(const Args a) {
                 for (int gp = 0; gp < 2; gp++)
 #pragma unroll
                     for (int blk = 0; blk < 2; blk++) {
-                        const float p0 = wt[2 * blk] * (gp ? high_elem<DT>(vs[2 * blk][w % WV]) : low_elem<DT>(vs[2 * blk][w % WV]));
-                        const float p1 = wt[2 * blk + 1] *
-                                         (gp ? high_elem<DT>(vs[2 * blk + 1][w % WV]) : low_elem<DT>(vs[2 * blk + 1][w % WV]));
-                        split_pair<true, FEW>(p0, p1, keep_lo, keep_hi, hi[gp][blk], lo[gp][blk]);
+                        if (BF16) {   // both rows' scales as a pair
+                            scale_pair<FEW>(ph[blk], px[blk], __byte_perm(vs[2 * blk][w % WV], vs[2 * blk + 1][w % WV], gp ? 0x7632 : 0x5410),
+                                            hi[gp][blk], lo[gp][blk]);
+                        } else {
+                            const float p0 = wt[2 * blk] * (gp ? high_elem<DT>(vs[2 * blk][w % WV]) : low_elem<DT>(vs[2 * blk][w % WV]));
+                            const float p1 = wt[2 * blk + 1] *
+                                             (gp ? high_elem<DT>(vs[2 * blk + 1][w % WV]) : low_elem<DT>(vs[2 * blk + 1][w % WV]));
+                            split_pair<true, FEW>(p0, p1, keep_lo, keep_hi, hi[gp][blk], lo[gp][blk]);
+                        }
                     }
                 // value codes of rows (4t, 4t + 1) and (4t + 2, 4t + 3): nibble pairs of the same element
                 uint32_t va[2][2][4];

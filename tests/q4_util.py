@@ -43,8 +43,10 @@ def scan(k: torch.Tensor, q: torch.Tensor):
 def attend(q, k, v, mask, scale):
     """q (H, G, D), k / v (H, n, D) float64, mask (H, n) -> out (H, G, D), lse (H, G) in 64 bits, with the tolerances of an
     fp32 computation that rounds `out` to q's type: a logit is off by at most D * 2^-22 of the magnitudes it sums, which
-    changes every weight by that factor; the weights enter the second product with 16 bits (2^-16); n terms are summed
-    in fp32 (n * 2^-23); exp2 and the final division add 2^-20."""
+    changes every weight by that factor; n terms are summed in fp32 (n * 2^-23); exp2 and the final division add 2^-20.
+    A weight p enters the second product as p s in two bf16 pieces: p = h + x with |x| <= 2^-8 p kept to 2^-8 of itself,
+    i.e. 2^-16 of p; p s = round(h s) + y with y = (h s - round(h s)) + x s, at most 2^-8 + 2^-8 of p s, rounded once, i.e.
+    2^-15 of p s.  Together 1.5 * 2^-15, below 2^-14."""
     n, D = k.shape[1], k.shape[2]
     x = torch.matmul(q.double(), k.transpose(1, 2)) * scale
     mag = torch.matmul(q.double().abs(), k.abs().transpose(1, 2)) * scale
@@ -60,7 +62,7 @@ def attend(q, k, v, mask, scale):
     lse[empty] = -math.inf
     eps = D * 2.0 ** -22 * (mag.amax(-1) if n else torch.zeros_like(lse))
     spread = torch.matmul(p, v.abs())
-    rel = (2.0 * eps + 2.0 ** -16 + n * 2.0 ** -23 + 2.0 ** -20).unsqueeze(-1)
+    rel = (2.0 * eps + 2.0 ** -14 + n * 2.0 ** -23 + 2.0 ** -20).unsqueeze(-1)
     tol_out = rel * spread + HALF_STEP[q.dtype] * (out.abs() + rel * spread) + 2.0 ** -25
     tol_lse = eps + n * 2.0 ** -23 + 2.0 ** -20 + lse.abs().nan_to_num(posinf=0.0) * 2.0 ** -22
     return out, lse, tol_out, tol_lse
