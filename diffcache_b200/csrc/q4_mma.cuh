@@ -91,6 +91,24 @@ __device__ __forceinline__ float high_elem(uint32_t w) {
     return DT == DC_BF16 ? __uint_as_float(w & 0xFFFF0000u) : elem_to_float<DT>(static_cast<uint16_t>(w >> 16));
 }
 
+// The same pairs as fp16 subnormals: nibble u is u * 2^-24 as it stands in the low bits, and u * 2^-20 four bits up, so one mask
+// is all a pair takes.  What is left of the encoding, 2^-24 or 2^-20 and the 8, goes into the other operand (odd pairs: a
+// sixteenth of it) and the sum the products start from (- 8 * 2^-24 of the other operand's sum).
+__device__ __forceinline__ void codes_subnormal(uint32_t w, uint32_t (&p)[4]) {
+    const uint32_t hi = w >> 8;
+    p[0] = w & 0x000F000Fu;
+    p[1] = w & 0x00F000F0u;
+    p[2] = hi & 0x000F000Fu;
+    p[3] = hi & 0x00F000F0u;
+}
+// d = a b + c with c left as it is
+__device__ __forceinline__ void mma_from(float (&d)[4], const float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};\n"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+
 // Powers of two that bring a vector whose largest magnitude is `top` to [2^14, 2^15) and back: a bf16 element is then exact
 // in fp16 unless it is more than 2^31 times smaller than the largest.
 __device__ __forceinline__ void q4_normalise(float top, float& down, float& up) {

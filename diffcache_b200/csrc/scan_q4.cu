@@ -92,16 +92,25 @@ q4_scan_kernel(const Q4Rows keys, int64_t prob_rows, int64_t n, const int32_t* _
 
     // query fragments: column g of B holds group g, i.e. only the products with that group's codes are not zero
     uint32_t qb[D / 16][2];
+    float q_sum = 0.0f;                        // of column g, over this lane's rows of B
 #pragma unroll
     for (int c = 0; c < 2; c++)
 #pragma unroll
         for (int e = 0; e < 2; e++) {
             const int d = 32 * (g % NG) + 2 * (2 * t + c) + e;   // + 16: the group's other tile
-            const uint32_t v = pack2<false>(s_q[d] * down, s_q[d + 16] * down);
+            const float f = e ? down * 0.0625f : down;
+            const uint32_t v = pack2<false>(s_q[d] * f, s_q[d + 16] * f);
+            const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&v));
+            q_sum += (r.x + r.y) * (e ? 16.0f : 1.0f);
 #pragma unroll
             for (int i = 0; i < NG; i++) qb[2 * i + c][e] = g == i ? v : 0u;
         }
-    const CodeConst cc(static_cast<uint32_t>(rows_per_cta) >> 31);
+    q_sum += __shfl_xor_sync(0xFFFFFFFFu, q_sum, 1);
+    q_sum += __shfl_xor_sync(0xFFFFFFFFu, q_sum, 2);
+    // the sums start from - 8 * 2^-24 times their column's query sum (columns 2t, 2t + 1 of this lane)
+    const float start0 = -0x1p-21f * __shfl_sync(0xFFFFFFFFu, q_sum, 8 * t), start1 = -0x1p-21f * __shfl_sync(0xFFFFFFFFu, q_sum, 8 * t + 4);
+    const float start[4] = {2 * t < NG ? start0 : 0.0f, 2 * t < NG ? start1 : 0.0f, 2 * t < NG ? start0 : 0.0f, 2 * t < NG ? start1 : 0.0f};
+    up *= 0x1p24f;
 
     uint32_t* out = scores + prob * score_stride;
     uint32_t lo = 0xFFFFFFFFu, hi = 0u;
@@ -115,9 +124,9 @@ q4_scan_kernel(const Q4Rows keys, int64_t prob_rows, int64_t n, const int32_t* _
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
                     uint32_t p[4], r[4];
-                    codes_f16(cc, x.k[i][0][c * W + w], p);
-                    codes_f16(cc, x.k[i][1][c * W + w], r);
-                    if (w == 0 && c == 0) mma_first<false>(acc, p[0], r[0], p[1], r[1], qb[0][0], qb[0][1]);
+                    codes_subnormal(x.k[i][0][c * W + w], p);
+                    codes_subnormal(x.k[i][1][c * W + w], r);
+                    if (w == 0 && c == 0) mma_from(acc, start, p[0], r[0], p[1], r[1], qb[0][0], qb[0][1]);
                     else mma<false>(acc, p[0], r[0], p[1], r[1], qb[4 * w + c][0], qb[4 * w + c][1]);
                     mma<false>(acc, p[2], r[2], p[3], r[3], qb[4 * w + 2 + c][0], qb[4 * w + 2 + c][1]);
                 }
