@@ -2,10 +2,10 @@
 // and log-sum-exp merge: the 4-bit counterpart of attend.cu (flash_attn_with_kvcache over the gathered buffer,
 // src/diffcache/base.py:134-142), over the rows of an id list or over every stored row of a sequence.
 //
-// Bound, at head_dim 128 and four query heads: 144 bytes a row against 407 instructions per 16 rows, most of them turning
-// nibbles into fragment values.  64 problems x 32768 consecutive rows: 79 us = 3.8 TB/s of codes and scales, 2.7 instructions
+// Bound, at head_dim 128 and four query heads: 144 bytes a row against about 385 instructions per 16 rows, most of them turning
+// nibbles into fragment values.  64 problems x 32768 consecutive rows: 76 us = 4.0 TB/s of codes and scales, 2.7 instructions
 // per clock (operands loaded to registers without the ring: 116; keys as the columns of B instead of the rows of A: 110;
-// weights scaled and split in fp32: 83).  16384 random rows each: 65 us, 4.7 TB/s of DRAM traffic, twice the bytes used.
+// weights scaled and split in fp32, keys as fp16 integers with their offset subtracted: 83).  16384 random rows each: 65 us, 4.7 TB/s of DRAM traffic, twice the bytes used.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -195,8 +195,8 @@ __device__ __forceinline__ void transpose_weights(const float (&x)[4], float (&y
 // grid = (n_split, n_prob, ceil(group / 8)).
 //
 // Store rows.  S^T = K Q^T with m16n8k16 MMAs: 16 store rows are the rows of A, up to 8 query heads the columns of B.  The
-// codes enter as small integers (fp16, exact), so a group's partial product is exact up to fp32 accumulation and its scale
-// is applied once, in fp32.  The query of a head is normalised by a power of two so that a bf16 query is exact in fp16 too.
+// codes enter as small integers (fp16 subnormals, exact: codes_subnormal), so a group's partial product is exact up to fp32
+// accumulation and its scale is applied once, in fp32.  The query of a head is normalised by a power of two so that a bf16 query is exact in fp16 too.
 // O^T = V^T P^T: the value codes are A (16 elements of a tile x 16 rows, bf16 integers), the weights are B; a value's scale
 // depends on (row, group) only, so it multiplies the weight, which enters as a bf16 value and its remainder
 // (scale_pair for bf16 scales, split_pair for the 11 bits of fp16 ones).  With at most four heads value and remainder are two column groups of ONE MMA (columns h and h + 4),
@@ -368,20 +368,31 @@ q4_attend_kernel(const Args a) {
         top = __vmaxu2(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
         float down, up_g;
         q4_normalise(elem_to_float<DT>(static_cast<uint16_t>(max(top & 0xFFFFu, top >> 16))), down, up_g);
-        up_g *= a.scale_log2;
+        up_g *= a.scale_log2 * 0x1p24f;
         const float up[2] = {__shfl_sync(0xFFFFFFFFu, up_g, 8 * t), __shfl_sync(0xFFFFFFFFu, up_g, 8 * t + 4)};   // heads 2t, 2t + 1
         uint32_t qa[NT][2];
+        float start[NG][2];                            // where the sums of a group start: heads 2t, 2t + 1
 #pragma unroll
         for (int w = 0; w < D / 64; w++)
 #pragma unroll
-            for (int gp = 0; gp < 2; gp++)
+            for (int gp = 0; gp < 2; gp++) {
+                float sum = 0.0f;                      // of head g over this lane's part of the group
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
                     const int d = 16 * (4 * w + 2 * gp) + 2 * (2 * t + c);   // a tile's element; + 16 is the group's other tile
                     const uint32_t w0 = *reinterpret_cast<const uint32_t*>(qrow + d), w1 = *reinterpret_cast<const uint32_t*>(qrow + d + 16);
-                    qa[4 * w + 2 * gp + c][0] = pack2<false>(low_elem<DT>(w0) * down, low_elem<DT>(w1) * down);
-                    qa[4 * w + 2 * gp + c][1] = pack2<false>(high_elem<DT>(w0) * down, high_elem<DT>(w1) * down);
+                    uint32_t (&q)[2] = qa[4 * w + 2 * gp + c];
+                    q[0] = pack2<false>(low_elem<DT>(w0) * down, low_elem<DT>(w1) * down);
+                    q[1] = pack2<false>(high_elem<DT>(w0) * down * 0.0625f, high_elem<DT>(w1) * down * 0.0625f);
+                    const float2 r0 = __half22float2(*reinterpret_cast<const __half2*>(&q[0]));
+                    const float2 r1 = __half22float2(*reinterpret_cast<const __half2*>(&q[1]));
+                    sum += (r0.x + r0.y) + 16.0f * (r1.x + r1.y);
                 }
+                sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
+                sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
+                start[2 * w + gp][0] = -0x1p-21f * __shfl_sync(0xFFFFFFFFu, sum, 8 * t);
+                start[2 * w + gp][1] = -0x1p-21f * __shfl_sync(0xFFFFFFFFu, sum, 8 * t + 4);
+            }
 
         const CodeConst cc(static_cast<uint32_t>(a.kv_heads) >> 31);
         auto compute = [&](unsigned st, uint32_t ok) {
@@ -409,12 +420,15 @@ q4_attend_kernel(const Args a) {
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
                         uint32_t p[4], r[4];
-                        codes_f16(cc, kw[0][c * (D / 64) + w], p);
-                        codes_f16(cc, kw[1][c * (D / 64) + w], r);
+                        codes_subnormal(kw[0][c * (D / 64) + w], p);
+                        codes_subnormal(kw[1][c * (D / 64) + w], r);
 #pragma unroll
                         for (int gp = 0; gp < 2; gp++) {
                             const uint32_t (&q)[2] = qa[4 * w + 2 * gp + c];
-                            if (c == 0) mma_first<false>(acc[gp], p[2 * gp], r[2 * gp], p[2 * gp + 1], r[2 * gp + 1], q[0], q[1]);
+                            if (c == 0) {
+                                const float s4[4] = {start[2 * w + gp][0], start[2 * w + gp][1], start[2 * w + gp][0], start[2 * w + gp][1]};
+                                mma_from(acc[gp], s4, p[2 * gp], r[2 * gp], p[2 * gp + 1], r[2 * gp + 1], q[0], q[1]);
+                            }
                             else mma<false>(acc[gp], p[2 * gp], r[2 * gp], p[2 * gp + 1], r[2 * gp + 1], q[0], q[1]);
                         }
                     }

@@ -46,28 +46,15 @@ __device__ __forceinline__ void ldg_words(uint32_t (&r)[N], const void* p) {
 // Constants of the code conversion, kept in registers: with an immediate operand the packed 16-bit subtraction issues to
 // the integer pipe, which the masks already fill, instead of the FMA pipe.
 struct CodeConst {
-    uint32_t f16_one, f16_off, f16_16th, f16_off16, bf16_one, bf16_off;
+    uint32_t bf16_one, bf16_off;
     __device__ __forceinline__ explicit CodeConst(uint32_t zero) {   // 0, in a form the compiler cannot fold
-        f16_one = 0x64006400u | zero;    // 1024, 1024
-        f16_off = 0xE408E408u | zero;    // -1032
-        f16_16th = 0x2C002C00u | zero;   // 1 / 16
-        f16_off16 = 0xD480D480u | zero;  // -72
         bf16_one = 0x43004300u | zero;   // 128, 128
         bf16_off = 0xC308C308u | zero;   // -136
     }
 };
 
-// Four pairs of codes of a word: pair j = (nibble j, nibble j + 4).  Inserting a nibble into the mantissa of 1024 (fp16) or
-// 128 (bf16) makes it that number plus the nibble, exactly; the offset and the 8 of the encoding go with one operation.
-__device__ __forceinline__ void codes_f16(const CodeConst& k, uint32_t w, uint32_t (&p)[4]) {
-    const uint32_t hi = w >> 8;
-    const uint32_t t[4] = {(w & 0x000F000Fu) | k.f16_one, (w & 0x00F000F0u) | k.f16_one, (hi & 0x000F000Fu) | k.f16_one,
-                           (hi & 0x00F000F0u) | k.f16_one};
-    asm("add.f16x2 %0, %1, %2;\n" : "=r"(p[0]) : "r"(t[0]), "r"(k.f16_off));
-    asm("fma.rn.f16x2 %0, %1, %2, %3;\n" : "=r"(p[1]) : "r"(t[1]), "r"(k.f16_16th), "r"(k.f16_off16));
-    asm("add.f16x2 %0, %1, %2;\n" : "=r"(p[2]) : "r"(t[2]), "r"(k.f16_off));
-    asm("fma.rn.f16x2 %0, %1, %2, %3;\n" : "=r"(p[3]) : "r"(t[3]), "r"(k.f16_16th), "r"(k.f16_off16));
-}
+// Four pairs of codes of a word as bf16: pair j = (nibble j, nibble j + 4).  Inserting a nibble into the mantissa of 128 makes
+// it 128 plus the nibble, exactly; the offset and the 8 of the encoding go with one addition.
 __device__ __forceinline__ void codes_bf16(const CodeConst& k, uint32_t w, uint32_t (&p)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {

@@ -1,13 +1,14 @@
 // Score scan over keys held in 4 bits: the ranking keys of score_scan (scan.cu; nsw.rs:601-607 with QKDist,
 // nsw.rs:129-139) for stored keys s * c,  dist = 65536 - sum_g s_g * sum_{d in g} q_d c_d,  in fp32.
 //
-// 16 rows at a time go through m16n8k16 tensor-core products: the codes, as fp16 integers, are A; column j of B is the
+// 16 rows at a time go through m16n8k16 tensor-core products: the codes, as fp16 subnormals, are A; column j of B is the
 // query with every group but group j set to zero, so that ONE chain of head_dim / 16 products leaves the partial dot of
 // group j in column j, exact up to fp32 accumulation, and the scales are applied once per group in fp32.  The query is
 // normalised by a power of two, so that a bf16 query is exact in fp16 as well.  The codes come straight from global
 // memory to the fragment registers (the stored order makes a lane's share of a row contiguous), 64 rows per warp at a time.
-// Bound: HBM, 9/16 * head_dim bytes a row and 4 of output.  128 problems x 130496 rows of head_dim 128: 225 us = 5.65 TB/s (one
-// thread per row on the FMA pipe: 630 us; without the second register set 429; with 1024-row CTAs and the query first 325).
+// Bound: HBM, 9/16 * head_dim bytes a row and 4 of output.  128 problems x 130496 rows of head_dim 128: 208 us = 6.1 TB/s (one
+// thread per row on the FMA pipe: 630 us; without the second register set 429; with 1024-row CTAs and the query first 325;
+// with the codes converted to integers before the products 225).
 #include <algorithm>
 
 #include "q4_mma.cuh"
