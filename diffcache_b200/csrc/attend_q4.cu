@@ -368,7 +368,7 @@ q4_attend_kernel(const Args a) {
         top = __vmaxu2(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
         float down, up_g;
         q4_normalise(elem_to_float<DT>(static_cast<uint16_t>(max(top & 0xFFFFu, top >> 16))), down, up_g);
-        up_g *= a.scale_log2 * 0x1p24f;
+        up_g *= a.scale_log2;
         const float up[2] = {__shfl_sync(0xFFFFFFFFu, up_g, 8 * t), __shfl_sync(0xFFFFFFFFu, up_g, 8 * t + 4)};   // heads 2t, 2t + 1
         uint32_t qa[NT][2];
         float start[NG][2];                            // where the sums of a group start: heads 2t, 2t + 1
@@ -439,7 +439,7 @@ q4_attend_kernel(const Args a) {
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < 4; i++) sc[i] *= up[i & 1];
+                for (int i = 0; i < 4; i++) sc[i] = sc[i] * up[i & 1] * 0x1p24f;   // up * 2^24 may overflow
             }
             if (ok != 0xFFFFu) {   // rows that are not there: no weight (their scales and codes are zeros)
                 const int r = 4 * (g >> 1) + (g & 1);

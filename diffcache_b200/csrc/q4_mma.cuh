@@ -96,11 +96,11 @@ __device__ __forceinline__ void mma_from(float (&d)[4], const float (&c)[4], uin
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
-// Powers of two that bring a vector whose largest magnitude is `top` to [2^14, 2^15) and back: a bf16 element is then exact
-// in fp16 unless it is more than 2^31 times smaller than the largest.
+// Powers of two that bring a vector whose largest magnitude is `top` to [2^14, 2^15) and back: a bf16 element, and a sixteenth
+// of it, is then exact in fp16 unless it is more than 2^27 times smaller than the largest.
 __device__ __forceinline__ void q4_normalise(float top, float& down, float& up) {
     int ex = static_cast<int>((__float_as_uint(top) >> 23) & 255u);   // 0: zero or subnormal, 255: infinite
-    ex = ex == 255 ? 127 + 14 : max(ex, 28);
+    ex = ex == 255 ? 127 + 14 : max(ex, 15);   // the smallest for which both are normal numbers
     down = __uint_as_float(static_cast<uint32_t>(127 + 14 - ex + 127) << 23);   // 2^(14 - e)
     up = __uint_as_float(static_cast<uint32_t>(ex - 14) << 23);                 // 2^(e - 14)
 }

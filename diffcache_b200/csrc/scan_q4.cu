@@ -111,7 +111,6 @@ q4_scan_kernel(const Q4Rows keys, int64_t prob_rows, int64_t n, const int32_t* _
     // the sums start from - 8 * 2^-24 times their column's query sum (columns 2t, 2t + 1 of this lane)
     const float start0 = -0x1p-21f * __shfl_sync(0xFFFFFFFFu, q_sum, 8 * t), start1 = -0x1p-21f * __shfl_sync(0xFFFFFFFFu, q_sum, 8 * t + 4);
     const float start[4] = {2 * t < NG ? start0 : 0.0f, 2 * t < NG ? start1 : 0.0f, 2 * t < NG ? start0 : 0.0f, 2 * t < NG ? start1 : 0.0f};
-    up *= 0x1p24f;
 
     uint32_t* out = scores + prob * score_stride;
     uint32_t lo = 0xFFFFFFFFu, hi = 0u;
@@ -145,7 +144,7 @@ q4_scan_kernel(const Q4Rows keys, int64_t prob_rows, int64_t n, const int32_t* _
         for (int r = 0; r < 2; r++) {
             const int64_t row = base + 16 * t + 8 * r + g;
             if (t < kTiles && row < end) {
-                const uint32_t b = dist_bits(mine[r] * up);
+                const uint32_t b = dist_bits(mine[r] * up * 0x1p24f);   // up * 2^24 may overflow
                 out[row] = b;
                 lo = min(lo, b);
                 hi = max(hi, b);

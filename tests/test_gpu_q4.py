@@ -262,6 +262,26 @@ def test_score_rows_far_magnitudes(scale):
     q4_util.assert_close(bits.cpu().view(torch.float32).reshape(2, 200), dist, tol, "dist")
 
 
+@pytest.mark.parametrize("scale", [2.0 ** -119, 2.0 ** 115])
+def test_scores_and_attention_at_the_ends_of_the_range(scale):
+    """Keys near the smallest normal numbers with queries near the largest, and the other way round."""
+    x, y, q = _rows((1, 2, 200, 128), "bf16", 24, False), _rows((1, 2, 200, 128), "bf16", 25, False), _rows((1, 8, 128), "bf16", 26, False)
+    x, q = (x.double() * scale).to(x.dtype), (q.double() / scale).to(q.dtype)
+    eng = _engine(1, 2, 4, 128, 200)
+    eng.prefill(x.cuda(), y.cuda())
+    one = q[:, ::4].contiguous()
+    bits = torch.empty(1, 2, 200, dtype=torch.int32, device="cuda")
+    eng.score_rows(one.cuda(), bits)
+    ks, vs = q4_util.stored(x), q4_util.stored(y)
+    dist, tol = q4_util.scan(ks.reshape(2, 200, 128), one.reshape(2, 128))
+    q4_util.assert_close(bits.cpu().view(torch.float32).reshape(2, 200), dist, tol, "dist")
+    out, lse = torch.empty_like(q, device="cuda"), torch.empty(1, 8, device="cuda")
+    eng.attend_rows(q.cuda(), out, out_lse=lse)
+    want, wl, to, tl = q4_util.attend(q.reshape(2, 4, 128), ks[0], vs[0], torch.ones(2, 200, dtype=torch.bool), 128 ** -0.5)
+    q4_util.assert_close(out.cpu().reshape(2, 4, 128), want, to, "out")
+    q4_util.assert_close(lse.cpu().reshape(2, 4), wl, tl, "lse")
+
+
 # ---- attention ------------------------------------------------------------------------------------------------------
 
 def _attend_case(B, H, G, D, n, dtype, seed, ids=None, lens=None, res=0, new=False, scale=0.0, spread=False, prep=None):
