@@ -2,10 +2,10 @@
 // and log-sum-exp merge: the 4-bit counterpart of attend.cu (flash_attn_with_kvcache over the gathered buffer,
 // src/diffcache/base.py:134-142), over the rows of an id list or over every stored row of a sequence.
 //
-// Bound, at head_dim 128 and four query heads: 144 bytes a row against about 385 instructions per 16 rows, most of them turning
+// Bound, at head_dim 128 and four query heads: 144 bytes a row against 387 instructions per 16 rows, most of them turning
 // nibbles into fragment values.  64 problems x 32768 consecutive rows: 76 us = 4.0 TB/s of codes and scales, 2.7 instructions
 // per clock (operands loaded to registers without the ring: 116; keys as the columns of B instead of the rows of A: 110;
-// weights scaled and split in fp32, keys as fp16 integers with their offset subtracted: 83).  16384 random rows each: 65 us, 4.7 TB/s of DRAM traffic, twice the bytes used.
+// weights scaled and split in fp32, keys as fp16 integers with their offset subtracted: 83).  16384 random rows each: 63 us, 4.8 TB/s of DRAM traffic, twice the bytes used.
 #include <cooperative_groups.h>
 
 #include <algorithm>
