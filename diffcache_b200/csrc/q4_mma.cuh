@@ -80,7 +80,9 @@ __device__ __forceinline__ float high_elem(uint32_t w) {
 
 // The same pairs as fp16 subnormals: nibble u is u * 2^-24 as it stands in the low bits, and u * 2^-20 four bits up, so one mask
 // is all a pair takes.  What is left of the encoding, 2^-24 or 2^-20 and the 8, goes into the other operand (odd pairs: a
-// sixteenth of it) and the sum the products start from (- 8 * 2^-24 of the other operand's sum).
+// sixteenth of it) and the sum the products start from (- 8 * 2^-24 of the other operand's sum).  A sum then passes through values
+// of up to (|c| + 16) |q| per element instead of |c| |q|: its fp32 rounding is relative to those, about 2^-18 of what half a step of
+// the codes may change it by even where the codes themselves are small.
 __device__ __forceinline__ void codes_subnormal(uint32_t w, uint32_t (&p)[4]) {
     const uint32_t hi = w >> 8;
     p[0] = w & 0x000F000Fu;

@@ -282,6 +282,34 @@ def test_scores_and_attention_at_the_ends_of_the_range(scale):
     q4_util.assert_close(lse.cpu().reshape(2, 4), wl, tl, "lse")
 
 
+def test_scores_and_attention_where_the_large_channel_does_not_count():
+    """Every group has one channel 100 times the rest, which the query ignores: the codes that count are small.  The 32-bit
+    sums take codes with an offset of 8 and take it back, so their magnitudes are up to (|c| + 16) |q| s an element, and
+    the bound of 2^-22 a step holds for those: 16 |q| s more than where only |c| |q| s are summed."""
+    B, H, G, D, n = 1, 2, 4, 128, 300
+    x, y, q = _rows((B, H, n, D), "bf16", 27, False), _rows((B, H, n, D), "bf16", 28, False), _rows((B, H * G, D), "bf16", 29, False)
+    x[..., ::32] *= 100
+    q[..., ::32] = 0
+    eng = _engine(B, H, G, D, n)
+    eng.prefill(x.cuda(), y.cuda())
+    one = q[:, ::G].contiguous()
+    bits = torch.empty(B, H, n, dtype=torch.int32, device="cuda")
+    eng.score_rows(one.cuda(), bits)
+    ks, vs = q4_util.stored(x), q4_util.stored(y)
+    steps = q4_util.quantise(x)[1].expand(B, H, n, D // 32, 32).reshape(H, n, D)
+    dist, tol = q4_util.scan(ks.reshape(H, n, D), one.reshape(H, D))
+    more = 16 * D * 2.0 ** -22 * torch.matmul(steps, one.reshape(H, D, 1).double().abs()).squeeze(-1)
+    q4_util.assert_close(bits.cpu().view(torch.float32).reshape(H, n), dist, tol + more, "dist")
+    out, lse = torch.empty_like(q, device="cuda"), torch.empty(B, H * G, device="cuda")
+    eng.attend_rows(q.cuda(), out, out_lse=lse)
+    qh = q.reshape(H, G, D)
+    want, wl, to, tl = q4_util.attend(qh, ks[0], vs[0], torch.ones(H, n, dtype=torch.bool), D ** -0.5)
+    more = 16 * D * 2.0 ** -22 * D ** -0.5 * torch.matmul(qh.double().abs(), steps.transpose(1, 2)).amax(-1)
+    q4_util.assert_close(lse.cpu().reshape(H, G), wl, tl + more, "lse")
+    to = to + 2.02 * more.unsqueeze(-1) * vs[0].abs().amax(1, keepdim=True)     # every weight off by that factor, |v| at most its largest
+    q4_util.assert_close(out.cpu().reshape(H, G, D), want, to, "out")
+
+
 # ---- attention ------------------------------------------------------------------------------------------------------
 
 def _attend_case(B, H, G, D, n, dtype, seed, ids=None, lens=None, res=0, new=False, scale=0.0, spread=False, prep=None):
